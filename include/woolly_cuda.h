@@ -43,7 +43,7 @@ typedef enum wl_status {
 } wl_status;
 
 /* GGML tensor type ids (crates/woolly-gguf/src/tensor_info.rs:15-60). */
-enum { WL_F32 = 0, WL_F16 = 1, WL_Q4_0 = 2, WL_Q4_1 = 3, WL_Q8_0 = 8, WL_Q4_K = 12, WL_Q6_K = 14 };
+enum { WL_F32 = 0, WL_F16 = 1, WL_Q4_0 = 2, WL_Q4_1 = 3, WL_Q8_0 = 8, WL_Q4_K = 12, WL_Q6_K = 14, WL_BF16 = 30 };
 
 /* Weight layouts.  LAYOUT_A is ggml's row-major [rows][K/32 blocks] used by
  * woolly-tensor's quantized_matvec (quantization.rs:1100-1163).  LAYOUT_B is
@@ -298,6 +298,148 @@ int wl_rope(const float* x, float* out, const int* positions, float base, int ba
  * attends keys (pos-window, pos] (window 0 = full prefix). out [rows, H*hd]. */
 int wl_attention(const float* q, const float* k, const float* v, int rows, int past,
                  int heads, int kv_heads, int head_dim, int window, float* out, void* stream);
+
+/* ------------------------------------------------------------------ */
+/* A serving step on a paged KV cache that the caller holds (device pointers,
+ * stream-ordered, no allocation, no host copies; capturable in a CUDA graph).
+ * No counterpart in the reference, which serves one request at a time.
+ * Pages hold 16 tokens; a cache is [pages][kv_heads][16][head_dim], the layout
+ * of the runtime's own.  Token p of request i lies in page tables[i][p / 16]
+ * and its slot is page * 16 + p % 16. */
+
+/* what became of a request (wl_step_plan.status, wl_release_result.status) */
+enum {
+  WL_STEP_OK = 0,
+  WL_STEP_NO_PAGES = 1,    /* the free list is used up (release: has no room) */
+  WL_STEP_TABLE_FULL = 2,  /* more tokens than the table row has pages for
+                              (release: the table holds no page there) */
+  WL_STEP_NO_ROWS = 3,     /* its rows do not fit */
+  WL_STEP_BAD_REQUEST = 4  /* a negative length or count, or more drafted
+                              tokens than the mask has bits */
+};
+
+typedef struct wl_step_plan {
+  int* row_start;     /* [n + 1] first row of each request */
+  int* requests;      /* [rows] the row's request, -1 behind the last */
+  int* positions;     /* [rows] the row's position, -1 for a row left out */
+  int* slots;         /* [rows] the row's slot in the cache, -1 for a row left out */
+  int* lengths;       /* [n] tokens held after the step (may be `lengths`) */
+  int* status;        /* [n] WL_STEP_* */
+  int* free_count;    /* [1] free pages left (may be `free_count`) */
+  int* page_start;    /* [n + 1] pages taken by the requests before each */
+  uint32_t* mask;     /* [rows][words] with parents, else unused */
+} wl_step_plan;
+
+/* Block tables, slot maps and positions of a step in which request i, holding
+ * lengths[i] tokens, adds counts[i] (0 and more).  tables [n][ld_tables] (max_pages
+ * entries a row are used) gets the new pages, taken in request order from the
+ * top of the stack free_pages[0 .. *free_count) of free_cap entries, which
+ * itself is only read.  Requests are served in order until the first one that
+ * the stack has too few pages for; that one and later ones that need pages are
+ * not (WL_STEP_NO_PAGES), requests that need none still are.  A request that
+ * is not served keeps its rows in row_start but takes no page: its rows have
+ * slot and position -1.  row_start never passes `rows`, the size of the row
+ * arrays; rows behind the last request get -1 throughout.
+ * With parents [rows] the rows of a request are a tree of drafted tokens:
+ * parents[r] is the index of an earlier node of the same request, or -1 for
+ * children of the last cached token.  positions then count the depth, and bit
+ * c % 32 of mask[r][c / 32] says that node c is r's own node or one of its
+ * ancestors (32 * words bits).  A row whose path meets a parent that is not an
+ * earlier node gets slot and position -1 and an empty mask. */
+int wl_block_tables(int* tables, int ld_tables, int max_pages, const int* lengths, const int* counts, int n,
+                    const int* free_pages, int free_cap, const int* free_count, int rows, const int* parents,
+                    int words, const wl_step_plan* out, void* stream);
+
+typedef struct wl_release_result {
+  int* lengths;    /* [n] tokens held afterwards (may be `lengths`) */
+  int* status;     /* [n] WL_STEP_* */
+  int* free_count; /* [1] (may be `free_count`) */
+  int* page_start; /* [n + 1] pages given back by the requests before each */
+} wl_release_result;
+
+/* Request i keeps its first min(keep[i], lengths[i]) tokens; the pages past
+ * them go back to the stack, and their table entries become -1.  Releasing
+ * what a step took leaves the stack as it was.  Requests are served in order
+ * while the stack has room. */
+int wl_release_pages(int* tables, int ld_tables, int max_pages, const int* lengths, const int* keep, int n,
+                     int* free_pages, int free_cap, const int* free_count, const wl_release_result* out,
+                     void* stream);
+
+/* K and V rows [rows][kv_heads * head_dim] (row strides ldk, ldv in elements)
+ * into their slots; slots outside the cache are skipped.  src_type f32 with an
+ * f16 or bf16 cache (rounded to nearest), or the cache's own type.  head_dim %
+ * 8 == 0; rows and caches 16-byte aligned.  The slots of one call are
+ * distinct: where two rows name one, either may end there. */
+int wl_kv_append(int src_type, int cache_type, const void* k, const void* v, size_t ldk, size_t ldv,
+                 const int* slots, int rows, int kv_heads, int head_dim, int n_pages, void* cache_k,
+                 void* cache_v, void* stream);
+
+/* Accepted drafts move together: with accepted[accepted_start[i] + j] the
+ * nodes that request i keeps, in rising order, the K and V of token
+ * lengths[i] + node go to token lengths[i] + j.  n_accepted is the size of
+ * `accepted`.  f16 or bf16 caches; head_dim % 8 == 0, at most 1024. */
+int wl_kv_commit(int cache_type, const int* tables, int ld_tables, int max_pages, const int* lengths, int n,
+                 const int* accepted, const int* accepted_start, int n_accepted, int kv_heads, int head_dim,
+                 int n_pages, void* cache_k, void* cache_v, void* stream);
+
+/* GQA attention (lazy_transformer.rs:375-434) of ragged rows over the cache:
+ * rows row_start[i] .. row_start[i + 1] of q [rows][ldq] are request i's
+ * tokens, whose K and V lie behind its lengths[i] cached ones (wl_kv_append at
+ * wl_block_tables' slots; `lengths` are those given to it).  A row attends the
+ * cached tokens and the step's own tokens named by its mask bits (its own
+ * among them); without a mask the earlier tokens of its request and itself.
+ * window > 0 keeps keys at positions > positions[r] - window.  Rows with a
+ * negative position, and rows with nothing to attend, give zeros; rows behind
+ * row_start[n] are left as they were.  Keys on pages outside the cache are
+ * masked.  q and out are f32 over an f16 cache, or f16 / bf16 over a cache of
+ * the same type; head_dim 32, 64, 128 or 256.  workspace: wl_tree_attention_workspace
+ * bytes of device memory, 16-byte aligned, which the call uses alone until it
+ * has finished. */
+size_t wl_tree_attention_workspace(int q_type, int n, int rows, int heads, int kv_heads, int head_dim);
+int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k, const void* cache_v,
+                      int n_pages, const int* tables, int ld_tables, int max_pages, const int* lengths,
+                      const int* row_start, const int* positions, const uint32_t* mask, int words, int n,
+                      int rows, int heads, int kv_heads, int head_dim, int window, float scale, void* out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rules on logits before sampling, per row r of [rows][vocab] (f32, f16 or
+ * bf16; row strides ld, ldo; out may be logits).  With n_v the times token v
+ * occurs among the tokens that the row's request produced, and v "seen" when
+ * it occurs there or in the prompt:
+ *   y = seen ? (x > 0 ? x / repetition : x * repetition) : x
+ *   y -= frequency * n_v + presence * (n_v > 0)
+ *   y += bias of v       y = -inf where the row's mask has bit v clear
+ * computed in f32 and rounded once.  Produced tokens are those of the request's
+ * history behind its first prompt_lens tokens and, for drafted rows, the tokens
+ * of the row's path.  Every group of pointers may be null: */
+typedef struct wl_logit_params {
+  float repetition; /* 1 = off; > 0 */
+  float presence, frequency;
+  int allowed_row; /* row of `allowed` that holds for this row of logits, -1 = none */
+} wl_logit_params;
+typedef struct wl_logit_context {
+  /* histories: tokens history[history_start[h] .. history_start[h + 1]) of
+   * request h < n_history; history_total is the size of `history` */
+  const int *history, *history_start, *prompt_lens;
+  int n_history, history_total;
+  const int* requests;        /* [rows] the row's request (null: row r is request r) */
+  /* drafted rows (wl_block_tables): node c of the row's path is draft_tokens[row_start[request] + c] */
+  const int* draft_tokens;    /* [rows] */
+  const uint32_t* draft_mask; /* [rows][words] */
+  int words;
+  const int* row_start;       /* [n_history + 1] */
+  /* biases of row r: entries bias_start[r] .. bias_start[r + 1); of several
+   * for one token the last holds; bias_total is their number */
+  const int *bias_start, *bias_tokens;
+  const float* bias_values;
+  int bias_total;
+  /* masks: bit v % 32 of allowed[m][v / 32] set = token v may follow */
+  const uint32_t* allowed;
+  int n_allowed, allowed_words;
+} wl_logit_context;
+int wl_process_logits(int type, const void* logits, size_t ld, int rows, int vocab,
+                      const wl_logit_params* params, const wl_logit_context* ctx, void* out, size_t ldo,
+                      void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Model runtime.  Replaces LazyTransformer (woolly-core model/lazy_transformer.rs)

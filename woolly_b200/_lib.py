@@ -31,9 +31,12 @@ WL_ERR_TIMEOUT = 15
 
 F32, F16, Q4_0, Q4_1, Q8_0 = 0, 1, 2, 3, 8
 Q4_K, Q6_K = 12, 14
+BF16 = 30
 LAYOUT_A, LAYOUT_B = 0, 1
 ROPE_OFF, ROPE_NEOX = 0, 1
 LOGITS_LAST, LOGITS_ALL = 0, 1
+# what became of a request of a step (ops.block_tables, ops.release_pages)
+STEP_OK, STEP_NO_PAGES, STEP_TABLE_FULL, STEP_NO_ROWS, STEP_BAD_REQUEST = 0, 1, 2, 3, 4
 
 
 class WoollyError(RuntimeError):
@@ -81,6 +84,27 @@ class ModelOptions(C.Structure):
                 ("collective_timeout_ms", C.c_int)]
 
 
+class StepPlan(C.Structure):
+    """wl_step_plan: the output buffers of wl_block_tables."""
+    _fields_ = [(n, C.c_void_p) for n in ("row_start", "requests", "positions", "slots", "lengths",
+                                          "status", "free_count", "page_start", "mask")]
+
+
+class ReleaseResult(C.Structure):
+    """wl_release_result: the output buffers of wl_release_pages."""
+    _fields_ = [(n, C.c_void_p) for n in ("lengths", "status", "free_count", "page_start")]
+
+
+class LogitContext(C.Structure):
+    """wl_logit_context: histories, drafts, biases and masks of wl_process_logits."""
+    _fields_ = [("history", C.c_void_p), ("history_start", C.c_void_p), ("prompt_lens", C.c_void_p),
+                ("n_history", C.c_int), ("history_total", C.c_int), ("requests", C.c_void_p),
+                ("draft_tokens", C.c_void_p), ("draft_mask", C.c_void_p), ("words", C.c_int),
+                ("row_start", C.c_void_p), ("bias_start", C.c_void_p), ("bias_tokens", C.c_void_p),
+                ("bias_values", C.c_void_p), ("bias_total", C.c_int), ("allowed", C.c_void_p),
+                ("n_allowed", C.c_int), ("allowed_words", C.c_int)]
+
+
 P = C.c_void_p
 _SIGS = {
     "wl_last_error": (C.c_char_p, []),
@@ -120,6 +144,20 @@ _SIGS = {
     "wl_swiglu": (C.c_int, [P, P, C.c_size_t, P, P]),
     "wl_nccl_comm_abort": (C.c_int, [P]),
     "wl_sample": (C.c_int, [P, C.c_int, C.c_int, C.c_int, P, P, P]),
+    "wl_block_tables": (C.c_int, [P, C.c_int, C.c_int, P, P, C.c_int, P, C.c_int, P, C.c_int, P,
+                                  C.c_int, C.POINTER(StepPlan), P]),
+    "wl_release_pages": (C.c_int, [P, C.c_int, C.c_int, P, P, C.c_int, P, C.c_int, P,
+                                   C.POINTER(ReleaseResult), P]),
+    "wl_kv_append": (C.c_int, [C.c_int, C.c_int, P, P, C.c_size_t, C.c_size_t, P, C.c_int, C.c_int,
+                               C.c_int, C.c_int, P, P, P]),
+    "wl_kv_commit": (C.c_int, [C.c_int, P, C.c_int, C.c_int, P, C.c_int, P, P, C.c_int, C.c_int,
+                               C.c_int, C.c_int, P, P, P]),
+    "wl_tree_attention_workspace": (C.c_size_t, [C.c_int] * 6),
+    "wl_tree_attention": (C.c_int, [C.c_int, P, C.c_size_t, P, P, C.c_int, P, C.c_int, C.c_int, P, P,
+                                    P, P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                    C.c_int, C.c_float, P, P, C.c_size_t, P]),
+    "wl_process_logits": (C.c_int, [C.c_int, P, C.c_size_t, C.c_int, C.c_int, P,
+                                    C.POINTER(LogitContext), P, C.c_size_t, P]),
     "wl_rope": (C.c_int, [P, P, P, C.c_float, C.c_int, C.c_int, C.c_int, C.c_int, P]),
     "wl_attention": (C.c_int, [P, P, P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                P, P]),

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 #include <set>
@@ -506,6 +507,157 @@ int wl_attention(const float* q, const float* k, const float* v, int rows, int p
     return fail(WL_ERR_INVALID_ARGUMENT, "bad argument");
   return launch_attention_f32(q, k, v, rows, past, heads, kv_heads, head_dim, window, out,
                               (cudaStream_t)stream);
+}
+
+// ---------------- a serving step on a paged cache ----------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+constexpr int kMaxTablePages = 1 << 26;  // tokens of a request stay below 2^30
+
+int wl_block_tables(int* tables, int ld_tables, int max_pages, const int* lengths, const int* counts, int n,
+                    const int* free_pages, int free_cap, const int* free_count, int rows, const int* parents,
+                    int words, const wl_step_plan* out, void* stream) {
+  if (n < 0 || rows < 0 || free_cap < 0 || max_pages < 0 || ld_tables < max_pages || max_pages > kMaxTablePages)
+    return fail(WL_ERR_INVALID_ARGUMENT, "block_tables: bad size");
+  if (!out || !free_count || (free_cap && !free_pages) || (n && (!lengths || !counts || (max_pages && !tables))))
+    return fail(WL_ERR_INVALID_ARGUMENT, "block_tables: null pointer");
+  if (parents ? words < 1 || words > 1024 : rows && words != 0)
+    return fail(WL_ERR_INVALID_ARGUMENT, "block_tables: 1..1024 mask words with parents, none without");
+  if (!out->row_start || !out->page_start || !out->free_count || (n && (!out->lengths || !out->status)) ||
+      (rows && (!out->requests || !out->positions || !out->slots || (parents && !out->mask))))
+    return fail(WL_ERR_INVALID_ARGUMENT, "block_tables: null output");
+  if (n && out->lengths == counts) return fail(WL_ERR_INVALID_ARGUMENT, "block_tables: the new lengths may not lie on the counts");
+  PlanArgs a;
+  a.tables = tables, a.ld_tables = ld_tables, a.max_pages = max_pages;
+  a.lengths = lengths, a.counts = counts, a.n = n;
+  a.free_pages = free_pages, a.free_cap = free_cap, a.free_count = free_count;
+  a.rows = rows, a.parents = parents, a.words = words, a.out = *out;
+  return launch_block_tables(a, (cudaStream_t)stream);
+}
+
+int wl_release_pages(int* tables, int ld_tables, int max_pages, const int* lengths, const int* keep, int n,
+                     int* free_pages, int free_cap, const int* free_count, const wl_release_result* out,
+                     void* stream) {
+  if (n < 0 || free_cap < 0 || max_pages < 0 || ld_tables < max_pages || max_pages > kMaxTablePages)
+    return fail(WL_ERR_INVALID_ARGUMENT, "release_pages: bad size");
+  if (!out || !free_count || (free_cap && !free_pages) || (n && (!lengths || !keep || (max_pages && !tables))))
+    return fail(WL_ERR_INVALID_ARGUMENT, "release_pages: null pointer");
+  if (!out->page_start || !out->free_count || (n && (!out->lengths || !out->status)))
+    return fail(WL_ERR_INVALID_ARGUMENT, "release_pages: null output");
+  if (n && out->lengths == keep) return fail(WL_ERR_INVALID_ARGUMENT, "release_pages: the new lengths may not lie on keep");
+  ReleaseArgs a;
+  a.tables = tables, a.ld_tables = ld_tables, a.max_pages = max_pages;
+  a.lengths = lengths, a.keep = keep, a.n = n;
+  a.free_pages = free_pages, a.free_cap = free_cap, a.free_count = free_count, a.out = *out;
+  return launch_release_pages(a, (cudaStream_t)stream);
+}
+
+int wl_kv_append(int src_type, int cache_type, const void* k, const void* v, size_t ldk, size_t ldv,
+                 const int* slots, int rows, int kv_heads, int head_dim, int n_pages, void* cache_k,
+                 void* cache_v, void* stream) {
+  if (rows < 0 || n_pages < 0 || kv_heads <= 0 || head_dim <= 0 || head_dim % 8)
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_append: bad size (head_dim must be a multiple of 8)");
+  if ((long long)n_pages * kKvPage > 0x7fffffffLL || (long long)kv_heads * head_dim > (1 << 24))
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_append: the cache has more than 2^31 slots or too wide rows");
+  if (cache_type != WL_F16 && cache_type != WL_BF16) return fail(WL_ERR_UNSUPPORTED, "kv_append: f16 or bf16 caches");
+  if (rows == 0) return WL_OK;
+  if (!k || !v || !slots || (n_pages && (!cache_k || !cache_v)))
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_append: null pointer");
+  const size_t es = src_type == WL_F32 ? 4 : 2, width = (size_t)kv_heads * head_dim;
+  if (ldk < width || ldv < width) return fail(WL_ERR_INVALID_ARGUMENT, "kv_append: rows overlap");
+  if (!aligned16(k) || !aligned16(v) || ldk * es % 16 || ldv * es % 16 || !aligned16(cache_k) || !aligned16(cache_v))
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_append: rows and caches must be 16-byte aligned");
+  return launch_kv_append(src_type, cache_type, k, v, ldk, ldv, slots, rows, kv_heads, head_dim,
+                          n_pages * kKvPage, cache_k, cache_v, (cudaStream_t)stream);
+}
+
+int wl_kv_commit(int cache_type, const int* tables, int ld_tables, int max_pages, const int* lengths, int n,
+                 const int* accepted, const int* accepted_start, int n_accepted, int kv_heads, int head_dim,
+                 int n_pages, void* cache_k, void* cache_v, void* stream) {
+  if (n < 0 || n_accepted < 0 || n_pages < 0 || max_pages < 0 || ld_tables < max_pages ||
+      max_pages > kMaxTablePages || kv_heads <= 0 || kv_heads > 65535 || head_dim <= 0 || head_dim % 8 ||
+      head_dim > 1024)
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_commit: bad size (head_dim must be a multiple of 8, at most 1024)");
+  if (cache_type != WL_F16 && cache_type != WL_BF16) return fail(WL_ERR_UNSUPPORTED, "kv_commit: f16 or bf16 caches");
+  if (n == 0 || n_accepted == 0 || max_pages == 0 || n_pages == 0) return WL_OK;
+  if (!tables || !lengths || !accepted || !accepted_start || !cache_k || !cache_v)
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_commit: null pointer");
+  if (!aligned16(cache_k) || !aligned16(cache_v))
+    return fail(WL_ERR_INVALID_ARGUMENT, "kv_commit: caches must be 16-byte aligned");
+  return launch_kv_commit(tables, ld_tables, max_pages, lengths, n, accepted, accepted_start, n_accepted,
+                          kv_heads, head_dim, n_pages, cache_k, cache_v, (cudaStream_t)stream);
+}
+
+size_t wl_tree_attention_workspace(int q_type, int n, int rows, int heads, int kv_heads, int head_dim) {
+  if (n <= 0 || rows <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
+  return tree_attention_workspace(q_type, n, rows, heads, kv_heads, head_dim);
+}
+
+int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k, const void* cache_v,
+                      int n_pages, const int* tables, int ld_tables, int max_pages, const int* lengths,
+                      const int* row_start, const int* positions, const uint32_t* mask, int words, int n,
+                      int rows, int heads, int kv_heads, int head_dim, int window, float scale, void* out,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (q_type != WL_F32 && q_type != WL_F16 && q_type != WL_BF16)
+    return fail(WL_ERR_UNSUPPORTED, "tree_attention: queries must be f32, f16 or bf16");
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(WL_ERR_UNSUPPORTED, "tree_attention: head_dim must be 32, 64, 128 or 256");
+  if (n < 0 || rows < 0 || n_pages < 0 || max_pages < 0 || ld_tables < max_pages || max_pages > kMaxTablePages ||
+      kv_heads <= 0 || heads <= 0 || heads % kv_heads || heads > 65535 || window < 0 ||
+      (mask ? words < 1 || words > 1024 : rows && words != 0))
+    return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: bad size");
+  if ((long long)n_pages * kKvPage * kv_heads > 0x7fffffffLL)
+    return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: the cache has more than 2^31 (slot, head) rows");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: scale must be positive and finite");
+  if (rows == 0 || n == 0) return WL_OK;
+  if (!q || !out || !lengths || !row_start || !positions || (max_pages && !tables) || (n_pages && (!cache_k || !cache_v)))
+    return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: null pointer");
+  const size_t es = q_type == WL_F32 ? 4 : 2;
+  if (ldq < (size_t)heads * head_dim) return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: rows of q overlap");
+  if (!aligned16(q) || ldq * es % 16 || !aligned16(out) || !aligned16(cache_k) || !aligned16(cache_v) ||
+      !aligned16(workspace))
+    return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: q, out, caches and workspace must be 16-byte aligned");
+  TreeAttnArgs a;
+  a.q = q, a.ldq = ldq, a.q_type = q_type, a.cache_k = cache_k, a.cache_v = cache_v, a.n_pages = n_pages;
+  a.tables = tables, a.ld_tables = ld_tables, a.max_pages = max_pages, a.lengths = lengths;
+  a.row_start = row_start, a.pos = positions, a.mask = mask, a.words = words;
+  a.n = n, a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
+  a.window = window, a.scale = scale, a.out = out;
+  const size_t need = tree_attention_workspace(q_type, n, rows, heads, kv_heads, head_dim);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(WL_ERR_BUFFER_TOO_SMALL, "tree_attention: needs " + std::to_string(need) + " bytes of workspace, got " +
+                                             std::to_string(workspace ? workspace_bytes : 0));
+  a.workspace = workspace;
+  return launch_tree_attention(a, (cudaStream_t)stream);
+}
+
+int wl_process_logits(int type, const void* logits, size_t ld, int rows, int vocab,
+                      const wl_logit_params* params, const wl_logit_context* ctx, void* out, size_t ldo,
+                      void* stream) {
+  if (type != WL_F32 && type != WL_F16 && type != WL_BF16)
+    return fail(WL_ERR_UNSUPPORTED, "process_logits: logits must be f32, f16 or bf16");
+  if (rows < 0 || vocab <= 0 || vocab > (1 << 27) || ld < (size_t)vocab || ldo < (size_t)vocab)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: bad size");
+  if (!ctx) return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: null context");
+  if (rows == 0) return WL_OK;
+  const wl_logit_context& c = *ctx;
+  if (c.n_history < 0 || c.history_total < 0 || c.bias_total < 0 || c.n_allowed < 0)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: negative size");
+  if (c.history_start ? (!c.history && c.history_total > 0) : c.history || c.prompt_lens)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: a history needs its tokens and their starts");
+  if (c.draft_mask ? !c.draft_tokens || !c.row_start || c.words < 1 || c.words > 1024 : c.draft_tokens || c.words)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: drafts need tokens, mask (1..1024 words) and row_start");
+  if (c.bias_start ? c.bias_total > 0 && (!c.bias_tokens || !c.bias_values) : c.bias_tokens || c.bias_values)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: biases need starts, tokens and values");
+  if (c.allowed && c.allowed_words < (vocab + 31) / 32)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: masks need a bit for every token");
+  if (!logits || !out || !params) return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: null pointer");
+  if (out == logits && ld != ldo)
+    return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: in place needs equal row strides");
+  LogitArgs a;
+  a.logits = logits, a.out = out, a.type = type, a.rows = rows, a.vocab = vocab, a.ld = ld, a.ldo = ldo;
+  a.params = params, a.ctx = c;
+  return launch_logits(a, (cudaStream_t)stream);
 }
 
 // ---------------- runtime ----------------

@@ -77,6 +77,76 @@ constexpr int kSampleMaxVocab = 51200;
 int launch_sample(const float* logits, int rows, int V, int ld, const wl_sample_params* prm,
                   uint32_t* out, cudaStream_t st);
 
+// Block tables, slot maps and cache writes of a serving step (pages.cu)
+constexpr int kKvPage = 16;  // tokens per KV page
+struct PlanArgs {
+  int* tables = nullptr;  // [n][ld_tables], max_pages entries used
+  int ld_tables = 0, max_pages = 0;
+  const int* lengths = nullptr;
+  const int* counts = nullptr;
+  int n = 0;
+  const int* free_pages = nullptr;
+  int free_cap = 0;
+  const int* free_count = nullptr;
+  int rows = 0;
+  const int* parents = nullptr;  // [rows] or null
+  int words = 0;                 // mask words per row; 0 without parents
+  wl_step_plan out{};
+};
+int launch_block_tables(const PlanArgs& a, cudaStream_t st);
+struct ReleaseArgs {
+  int* tables = nullptr;
+  int ld_tables = 0, max_pages = 0;
+  const int* lengths = nullptr;
+  const int* keep = nullptr;
+  int n = 0;
+  int* free_pages = nullptr;
+  int free_cap = 0;
+  const int* free_count = nullptr;
+  wl_release_result out{};
+};
+int launch_release_pages(const ReleaseArgs& a, cudaStream_t st);
+int launch_kv_append(int src, int cache, const void* k, const void* v, size_t ldk, size_t ldv, const int* slots,
+                     int rows, int kvh, int hd, int n_slots, void* ck, void* cv, cudaStream_t st);
+int launch_kv_commit(const int* tables, int ld_tables, int max_pages, const int* lengths, int n,
+                     const int* accepted, const int* accepted_start, int total, int kvh, int hd, int n_pages,
+                     void* ck, void* cv, cudaStream_t st);
+
+// Attention of a step's rows over the paged cache (tree_attention.cu)
+struct TreeAttnArgs {
+  const void* q = nullptr;  // [rows][ldq], a row's heads packed
+  size_t ldq = 0;
+  int q_type = WL_F32;  // f32 (f16 cache), f16 or bf16 (cache of the same type)
+  const void* cache_k = nullptr;
+  const void* cache_v = nullptr;
+  int n_pages = 0;
+  const int* tables = nullptr;
+  int ld_tables = 0, max_pages = 0;
+  const int* lengths = nullptr;
+  const int* row_start = nullptr;
+  const int* pos = nullptr;
+  const unsigned* mask = nullptr;
+  int words = 0;
+  int n = 0, rows = 0, heads = 0, kv_heads = 0, head_dim = 0, window = 0;
+  float scale = 0.f;
+  void* out = nullptr;  // [rows][heads * head_dim]
+  void* workspace = nullptr;
+};
+size_t tree_attention_workspace(int q_type, int n, int rows, int heads, int kv_heads, int head_dim);
+int launch_tree_attention(const TreeAttnArgs& a, cudaStream_t st);
+
+// Rules on logits before sampling (logits.cu)
+struct LogitArgs {
+  const void* logits = nullptr;
+  void* out = nullptr;
+  int type = WL_F32;
+  int rows = 0, vocab = 0;
+  size_t ld = 0, ldo = 0;
+  const wl_logit_params* params = nullptr;
+  wl_logit_context ctx{};
+};
+int launch_logits(const LogitArgs& a, cudaStream_t st);
+
 // dst[r][t * cols + c] = src[t][r][c]: the rank-major blocks of an all-gather
 // of column shards back into whole rows
 int launch_gather_cols(const float* src, int T, int rows, int cols, float* dst, cudaStream_t st);
