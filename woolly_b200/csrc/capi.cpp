@@ -610,7 +610,8 @@ int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k
   if (!(scale > 0.f) || !std::isfinite(scale))
     return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: scale must be positive and finite");
   if (rows == 0 || n == 0) return WL_OK;
-  if (!q || !out || !lengths || !row_start || !positions || (max_pages && !tables) || (n_pages && (!cache_k || !cache_v)))
+  if (n_pages == 0) return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: the cache has no pages");
+  if (!q || !out || !lengths || !row_start || !positions || (max_pages && !tables) || !cache_k || !cache_v)
     return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: null pointer");
   const size_t es = q_type == WL_F32 ? 4 : 2;
   if (ldq < (size_t)heads * head_dim) return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: rows of q overlap");
@@ -622,7 +623,8 @@ int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k
   a.tables = tables, a.ld_tables = ld_tables, a.max_pages = max_pages, a.lengths = lengths;
   a.row_start = row_start, a.pos = positions, a.mask = mask, a.words = words;
   a.n = n, a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
-  a.window = window, a.scale = scale, a.out = out;
+  a.window = window < (1 << 30) ? window : 0;  // past every token: none
+  a.scale = scale, a.out = out;
   const size_t need = tree_attention_workspace(q_type, n, rows, heads, kv_heads, head_dim);
   if (need && (!workspace || workspace_bytes < need))
     return fail(WL_ERR_BUFFER_TOO_SMALL, "tree_attention: needs " + std::to_string(need) + " bytes of workspace, got " +

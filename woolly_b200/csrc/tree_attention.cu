@@ -7,12 +7,41 @@
 // q.k * scale, the window W keeps keys at positions > pos[r] - W, and
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(s_j - max s).
 // A row with nothing to attend, or with a negative position, gives zeros.
+//
+// k_tree_attn, tcgen05.  The (row, head of the group) pairs of a request and a
+// KV head are the rows of 128-row query tiles, so a K / V tile is read once for
+// all of them.  A work item is a run of key tiles for one or two query tiles;
+// the key tiles of all (request, KV head, query tiles) are laid end to end and
+// cut evenly over one CTA per SM, whatever the lengths, each CTA finding its
+// share from a prefix sum over the requests.  A run that is not a whole group
+// leaves unnormalised parts (o, m, l), which k_tree_combine merges.
+//   warp 8     brings K and V tiles in with TMA, a 16-token page at a time
+//              (its 64-column halves land in 128-byte-swizzled rows);
+//   warp 9     issues S = Q K^T into TMEM and O += P V (P from TMEM, V as the
+//              MN-major operand straight from its rows);
+//   warps 0-7  two softmax groups, a thread per query row: S from TMEM into
+//              registers, mask, running maximum and sum, P back over S.
+// The groups work on two streams, so that one's softmax runs under the other's
+// products: the two query tiles of a pair over the same keys or, for a single
+// query tile, even and odd key tiles, merged with the parts.  head_dim 256 has
+// room in TMEM for one O only: one stream, with S double-buffered.
+// The maximum that P is taken against follows the true one with a lag of up to
+// 2^6 (O is rescaled only past that), and P is scaled by 2^8 where it is f16, so
+// that it stays clear of both ends of the type; both factors cancel in o / l.
+// f32 queries enter as two f16 words (22 bits), and so does P, two products
+// each against the f16 cache; f16 and bf16 queries take P in their own type.
+// V rows of keys that no row may see (the end of the last page, a drafted node
+// that is left out) are zeroed in shared memory, since 0 * NaN is not 0.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
+#include <cstring>
 #include <string>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.cuh"
@@ -101,15 +130,856 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
   for (int e = 0, d = tid; d < hd; d += 128, e++) put(out + d, l > 0.f ? o[e] / l : 0.f);
 }
 
+
+// ---------------------------------------------------------------- tcgen05
+constexpr int kTaThreads = 320;
+constexpr int kTaSmem = 224 * 1024;   // query tiles, then the ring of K / V tiles
+constexpr int kTaLag = 6;             // log2 of the lag of the maximum
+
+template <int HD, class Q>
+struct Shape {
+  static constexpr bool kSplit = sizeof(Q) == 4;       // f32 queries as two f16 words
+  static constexpr int KT = HD == 256 ? 64 : 128;      // keys per tile
+  static constexpr int NS = HD == 256 ? 1 : 2;         // streams
+  static constexpr int kQTile = 128 * HD * 2;          // bytes of a query tile (one word)
+  static constexpr int kQBytes = kQTile * NS * (kSplit ? 2 : 1);
+  static constexpr int kSlot = KT * HD * 2;            // bytes of a K or V tile
+  static constexpr int kSlots = (kTaSmem - kQBytes) / kSlot;
+  static constexpr int kO = 256;                       // TMEM column of O; S at 0 and KT
+  static constexpr bool kBf16 = std::is_same<Q, __nv_bfloat16>::value;
+  static constexpr float kShift = kBf16 ? 0.f : 8.f;   // log2 of P's scale
+  static constexpr uint32_t kType = kBf16 ? (1u << 7) | (1u << 10) : 0u;
+  // D f32; N at bit 17 (/8), M at bit 24 (/16), bit 16: B is MN-major
+  static constexpr uint32_t kIdescS = (1u << 4) | kType | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
+  static constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
+};
+
+__device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// bounded wait; gives up at once when another role has
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  for (int it = 0; it < (1 << 22); it++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 63) == 63 && *failed) return false;
+  }
+  *failed = 1;
+  return false;
+}
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
+         (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+#define WL_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define WL_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+// 32 columns of this thread's TMEM lane (no wait)
+__device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : WL_R8(v, 0), WL_R8(v, 8), WL_R8(v, 16), WL_R8(v, 24)
+      : "r"(a));
+}
+__device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n" ::WL_I8(v, 0),
+      WL_I8(v, 8), WL_I8(v, 16), WL_I8(v, 24), "r"(a)
+      : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15};\n" ::WL_I8(v, 0),
+      WL_I8(v, 8), "r"(a)
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  uint32_t u;
+  memcpy(&u, &h, 4);
+  return u;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  uint32_t u;
+  memcpy(&u, &h, 4);
+  return u;
+}
+
+// A request as the attention sees it, and its share of the work: per KV head,
+// qt query tiles times kt key tiles.
+struct Req {
+  int row0, T, len, keys;  // keys: end of the tokens that exist
+  int tile0;               // first key tile (window)
+  int kt, qt;
+};
+template <int KT>
+__device__ __forceinline__ Req request(const TreeAttnArgs& a, int i) {
+  Req q;
+  q.row0 = max(a.row_start[i], 0);
+  q.T = min(a.row_start[i + 1], a.rows) - q.row0;
+  if (q.T < 0) q.T = 0;
+  const long long cap = (long long)a.max_pages * kKvPage;
+  q.len = (int)min((long long)max(a.lengths[i], 0), cap);
+  q.keys = (int)min((long long)q.len + q.T, cap);
+  q.tile0 = a.window > 0 && q.len >= a.window ? (q.len - a.window + 1) / KT : 0;
+  q.kt = max(1, (q.keys + KT - 1) / KT - q.tile0);
+  q.qt = (int)(((long long)q.T * (a.heads / a.kv_heads) + 127) / 128);
+  return q;
+}
+__device__ __forceinline__ long long units(const TreeAttnArgs& a, const Req& q) {
+  return (long long)a.kv_heads * q.qt * q.kt;
+}
+
+// A run of key tiles [a, b) of one group: KV head kvh, query tiles qt0 .. qt0 + w - 1
+struct Run {
+  int i, kvh, qt0, w, a, b;
+  bool first, whole;  // the CTA's first run; the whole group
+};
+
+// Walks the CTA's share [x, x1) of the laid-out key tiles; all threads alike.
+template <int HD, class Q>
+struct Walk {
+  using S = Shape<HD, Q>;
+  long long x0, x, x1, base;  // base: start of request i
+  int i;
+  Req q;
+  __device__ bool next(const TreeAttnArgs& args, Run& r) {
+    while (x < x1) {
+      while (x >= base + units(args, q)) {
+        base += units(args, q);
+        q = request<S::KT>(args, ++i);
+      }
+      const long long per = (long long)q.qt * q.kt;
+      const long long off = x - base;
+      r.kvh = (int)(off / per);
+      const long long y = off - r.kvh * per;
+      r.qt0 = (int)(y / ((long long)S::NS * q.kt)) * S::NS;
+      r.w = min(S::NS, q.qt - r.qt0);
+      const long long g0 = base + r.kvh * per + (long long)r.qt0 * q.kt;
+      const long long g1 = g0 + (long long)r.w * q.kt, e = min(x1, g1);
+      r.i = i;
+      r.a = (int)((x - g0) / r.w);
+      r.b = (int)((e - g0) / r.w);
+      r.first = x0 >= g0;
+      r.whole = r.a == 0 && r.b == q.kt;
+      x = e;
+      if (r.b > r.a) return true;
+    }
+    return false;
+  }
+};
+
+// Parts: [CTA][first / last run][stream][prow rows][HD] f32, then (m, l) of
+// each; one status word per CTA and the requests' prefix sums before them.
+struct Parts {
+  int* status;       // [ctas]
+  long long* start;  // [n + 1]
+  float* o;
+  float* ml;
+  int prow;          // rows kept of a 128-row tile
+};
+__host__ __device__ inline size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+__host__ inline int part_rows(int rows, int group) {
+  const long long m = (long long)rows * group;
+  return m < 128 ? (int)m : 128;
+}
+__host__ inline size_t part_bytes(int ctas, int n, int hd, int prow) {
+  return round256((size_t)ctas * 4) + round256((size_t)(n + 1) * 8) + (size_t)ctas * 4 * prow * (hd + 2) * 4;
+}
+__host__ inline Parts parts_at(void* ws, int ctas, int n, int hd, int prow) {
+  Parts p;
+  uint8_t* b = (uint8_t*)ws;
+  p.status = (int*)b;
+  p.start = (long long*)(b + round256((size_t)ctas * 4));
+  p.o = (float*)(b + round256((size_t)ctas * 4) + round256((size_t)(n + 1) * 8));
+  p.ml = p.o + (size_t)ctas * 4 * prow * hd;
+  p.prow = prow;
+  return p;
+}
+
+__device__ __forceinline__ void st4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+
+template <int HD, class Q>
+__global__ void __launch_bounds__(kTaThreads, 1)
+    k_tree_attn(const TreeAttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                const Parts parts) {
+  using S = Shape<HD, Q>;
+  using C = typename std::conditional<S::kSplit, __half, Q>::type;
+  constexpr int KT = S::KT, NS = S::NS, NSLOT = S::kSlots, ATOMS = HD / 64, PAGES = KT / kKvPage;
+  extern __shared__ uint8_t ta_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t s_bars[2 * NSLOT + 10];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_fail;
+  __shared__ long long s_scan[kTaThreads / 32], s_base;
+  __shared__ int s_req;
+  __shared__ float2 s_ml[128];
+  const uint32_t full = sptr(s_bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
+                 pbar = sbar + 16, dbar = pbar + 16, obar = dbar + 8, endbar = obar + 8, xfull = endbar + 8, xempty = xfull + 8;
+  const uint32_t qs = sptr(sm), ring = qs + S::kQBytes;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = a.heads / a.kv_heads;
+
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&s_tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int k = 0; k < NSLOT; k++) bar_init(full + 8 * k, 1), bar_init(empty + 8 * k, 1);
+    bar_init(qbar, 256);
+    for (int k = 0; k < 2; k++) bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 128);
+    bar_init(dbar, 1);
+    bar_init(obar, 1);
+    bar_init(endbar, 1);
+    bar_init(xfull, 128);
+    bar_init(xempty, 128);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    s_fail = 0;
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mv) : "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // this CTA's share of the key tiles: the total, then the request it starts in
+  Walk<HD, Q> walk;
+  {
+    auto block_sum = [&](long long v, long long& before) {  // the sum, and that of the threads before this one
+      long long x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = x;
+      __syncthreads();
+      long long w = 0, all = 0;
+      for (int k = 0; k < kTaThreads / 32; k++) {
+        if (k == warp) w = all;
+        all += s_scan[k];
+      }
+      before = w + x - v;
+      return all;
+    };
+    long long total = 0, before;
+    for (int i0 = 0; i0 < a.n; i0 += kTaThreads)
+      total += block_sum(i0 + tid < a.n ? units(a, request<KT>(a, i0 + tid)) : 0, before);
+    walk.x0 = walk.x = total * blockIdx.x / gridDim.x;
+    walk.x1 = total * (blockIdx.x + 1) / gridDim.x;
+    long long sum = 0;
+    for (int i0 = 0; i0 < a.n; i0 += kTaThreads) {
+      const int i = i0 + tid;
+      const long long u = i < a.n ? units(a, request<KT>(a, i)) : 0;
+      const long long all = block_sum(u, before);
+      before += sum;
+      if (walk.x >= before && walk.x < before + u) s_req = i, s_base = before;
+      if (blockIdx.x == 0 && i < a.n) parts.start[i] = before;
+      sum += all;
+    }
+    if (blockIdx.x == 0 && tid == 0) parts.start[a.n] = total;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = s_tmem;
+  if (walk.x < walk.x1) {
+    walk.i = s_req;
+    walk.base = s_base;
+    walk.q = request<KT>(a, walk.i);
+  }
+  Run run;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA
+    // tiles in the order the products use them: a pair of query tiles K0 V0 K1
+    // V1 ..., a single one K0 K1 V0 K2 V1 ...
+    uint32_t seq = 0;
+    const int rows_end = a.n_pages * a.kv_heads * kKvPage;  // past the cache: read as zeros
+    bool ok = true;
+    while (ok && walk.next(a, run)) {
+      const int nt = run.b - run.a;
+      const int* table = a.tables + (size_t)run.i * a.ld_tables;
+      auto load = [&](const CUtensorMap* map, int tile) {
+        if (!ok) return;
+        const int pg = (walk.q.tile0 + run.a + tile) * PAGES + lane;
+        int row = rows_end;
+        if (lane < PAGES && pg < a.max_pages && pg * kKvPage < walk.q.keys) {
+          const int id = table[pg];
+          if (id >= 0 && id < a.n_pages) row = (id * a.kv_heads + run.kvh) * kKvPage;
+        }
+        const uint32_t slot = seq % NSLOT, bar = full + 8 * slot;
+        if (seq >= NSLOT) ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * slot, (seq / NSLOT - 1) & 1, &s_fail));
+        if (!ok) return;
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)S::kSlot)
+                       : "memory");
+        __syncwarp();
+        if (lane < PAGES) {
+#pragma unroll
+          for (int h = 0; h < ATOMS; h++)
+            asm volatile(
+                "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+                "[%4];\n" ::"r"(ring + slot * S::kSlot + h * KT * 128 + lane * kKvPage * 128),
+                "l"(map), "r"(h * 64), "r"(row), "r"(bar)
+                : "memory");
+        }
+        __syncwarp();
+        seq++;
+      };
+      if (run.w == 2) {
+        for (int t = 0; t < nt; t++) load(&mk, t), load(&mv, t);
+      } else {
+        load(&mk, 0);
+        if (nt > 1) load(&mk, 1);
+        for (int t = 0; t < nt; t++) {
+          load(&mv, t);
+          if (t + 2 < nt) load(&mk, t + 2);
+        }
+      }
+    }
+    // every copy has landed before the CTA ends
+    for (uint32_t k = seq > NSLOT ? seq - NSLOT : 0; k < seq; k++) {
+      int dummy = 0;
+      bar_wait(full + 8 * (k % NSLOT), (k / NSLOT) & 1, &dummy);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ products
+    if (lane == 0) {
+      uint32_t seq = 0;          // tiles of the ring used up by earlier runs
+      uint32_t np[2] = {0, 0};   // P tiles taken from each buffer
+      uint32_t runs = 0;
+      bool ok = true;
+      while (ok && walk.next(a, run)) {
+        const int nt = run.b - run.a, pair = run.w == 2, nu = pair ? 2 * nt : nt;
+        // place in the ring's order of the K and V tile of unit u
+        auto k_at = [&](int u) { return pair ? (uint32_t)(u >> 1) * 2 : u < 2 ? (uint32_t)u : (uint32_t)(2 * u - 1); };
+        auto v_at = [&](int u) {
+          return pair ? (uint32_t)(u >> 1) * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt);
+        };
+        auto scores = [&](int u) {  // S[u % 2] = Q K^T
+          const uint32_t k = seq + k_at(u), slot = k % NSLOT;
+          if (!(ok = ok && bar_wait(full + 8 * slot, (k / NSLOT) & 1, &s_fail))) return;
+          fence_after();
+          const uint32_t kb = ring + slot * S::kSlot, qb = qs + (pair ? (u & 1) * S::kQTile : 0);
+          const uint32_t d = tmem + (u & 1) * KT;
+#pragma unroll
+          for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ks++) {
+              const uint32_t o = (ks >> 2) * 128 * 128 + (ks & 3) * 32, ok_ = (ks >> 2) * KT * 128 + (ks & 3) * 32;
+              mma_ss(d, sw128_desc(qb + w * NS * S::kQTile + o, 16, 1024), sw128_desc(kb + ok_, 16, 1024), S::kIdescS,
+                     w || ks ? 1u : 0u);
+            }
+          mma_commit(sbar + 8 * (u & 1));
+          if (!pair || (u & 1)) mma_commit(empty + 8 * slot);
+        };
+        if (!(ok = bar_wait(qbar, runs & 1, &s_fail))) break;
+        runs++;
+        fence_after();
+        scores(0);
+        if (nu > 1) scores(1);
+        for (int u = 0; ok && u < nu; u++) {
+          const int b = u & 1;
+          const uint32_t k = seq + v_at(u), slot = k % NSLOT;
+          ok = bar_wait(pbar + 8 * b, np[b]++ & 1, &s_fail) && bar_wait(full + 8 * slot, (k / NSLOT) & 1, &s_fail);
+          if (!ok) break;
+          fence_after();
+          const uint32_t vb = ring + slot * S::kSlot, d = tmem + S::kO + (NS == 2 ? b * HD : 0), p = tmem + b * KT;
+          const bool fresh = NS == 2 ? u < 2 : u == 0;
+#pragma unroll
+          for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
+#pragma unroll
+            for (int ks = 0; ks < KT / 16; ks++)
+              mma_ts(d, p + w * (KT / 2) + ks * 8, sw128_desc(vb + ks * 16 * 128, KT * 128, 1024), S::kIdescO,
+                     fresh && !w && !ks ? 0u : 1u);
+          if (!pair || b) mma_commit(empty + 8 * slot);
+          if (NS == 1) mma_commit(obar);
+          if (u + 2 < nu) scores(u + 2);
+        }
+        if (ok) mma_commit(dbar);
+        seq += 2 * nt;
+      }
+      if (!ok) {  // products in flight finish before TMEM is given back
+        mma_commit(endbar);
+        int dummy = 0;
+        bar_wait(endbar, 0, &dummy);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int t = warp >> 2, wt = tid & 127;                 // stream; row of its query tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float c = a.scale * 1.4426950408889634f;
+    uint32_t ns[2] = {0, 0}, runs = 0, no = 0, seq = 0;
+    uint32_t nx = 0;           // exchanges between the streams
+    bool ok = true;
+    auto wait_warp = [&](uint32_t bar, uint32_t parity) {  // the same answer for the whole warp
+      return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, &s_fail));
+    };
+    while (ok && walk.next(a, run)) {
+      const Req& rq = walk.q;
+      const int nt = run.b - run.a, pair = run.w == 2, nu = pair ? 2 * nt : nt;
+      // queries: thread e of 256 copies 16-byte pieces of the (row, head) pairs
+      {
+        const int m0 = run.qt0 * 128, mn = min(run.w * 128, rq.T * group - m0);
+        const Q* src = (const Q*)a.q + (size_t)run.kvh * group * HD;
+        for (int e = tid; e < mn * (HD / 8); e += 256) {
+          const int m = e / (HD / 8), ch = e - m * (HD / 8);
+          const int j = (m0 + m) / group, g = (m0 + m) - j * group;
+          const Q* p = src + (size_t)(rq.row0 + j) * a.ldq + (size_t)g * HD + ch * 8;
+          const int row = m & 127;
+          uint8_t* d = sm + (m >> 7) * S::kQTile + (ch >> 3) * 128 * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+          if constexpr (S::kSplit) {
+            const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
+            const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const __half h0 = __float2half_rn(f[2 * k]), h1 = __float2half_rn(f[2 * k + 1]);
+              const __half2 h = __halves2half2(h0, h1);
+              memcpy(&hi[k], &h, 4);
+              lo[k] = pack2(f[2 * k] - __half2float(h0), f[2 * k + 1] - __half2float(h1), __half());
+            }
+            *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(d + NS * S::kQTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          } else {
+            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(p);
+          }
+        }
+      }
+      fence_async();
+      fence_before();
+      bar_arrive(qbar);
+
+      const int m = (run.qt0 + (pair ? t : 0)) * 128 + wt;
+      const int j = m / group, g = m - j * group;
+      const bool live = m < rq.T * group;
+      const int row = rq.row0 + (live ? j : 0);
+      int pos = live ? a.pos[row] : -1;
+      if (pos >= 0 && pos < rq.len) pos = rq.len;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      // a page outside the cache: then every tile looks at its pages
+      const int* table = a.tables + (size_t)run.i * a.ld_tables;
+      bool holes = false;
+      {
+        const int p1 = min((rq.tile0 + run.b) * PAGES, (rq.keys + kKvPage - 1) / kKvPage);
+        for (int p = (rq.tile0 + run.a) * PAGES + lane; p < p1; p += 32) {
+          const int id = table[p];
+          holes |= id < 0 || id >= a.n_pages;
+        }
+        holes = __any_sync(0xffffffffu, holes);
+      }
+      float mx = -INFINITY, l = 0.f;
+      const int step = NS == 2 ? 2 : 1;
+      for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step) {
+        const int b = u & 1, tile = pair ? u >> 1 : u, key0 = (rq.tile0 + run.a + tile) * KT;
+        ok = wait_warp(sbar + 8 * b, ns[b]++ & 1);
+        if (!ok) break;
+        fence_after();
+        const uint32_t sp = tmem + lanes + b * KT;
+        float s[KT];
+        if (warp_live) {
+#pragma unroll
+          for (int k = 0; k < KT / 32; k++) tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s) + k * 32);
+          tm_wait_ld();
+          const bool plain = key0 + KT <= rq.len && !holes && (a.window <= 0 || key0 > pos - a.window) && pos >= 0;
+          if (!__all_sync(0xffffffffu, plain || !live)) {
+#pragma unroll
+            for (int k = 0; k < KT / 32; k++) {
+              const int k0 = key0 + 32 * k;
+              uint32_t see = 0;
+              if (pos >= 0) {
+                // cached tokens: a range
+                const int lo = a.window > 0 ? max(pos - a.window + 1 - k0, 0) : 0, hi = min(rq.len - k0, 32);
+                if (hi > lo) see = (hi >= 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+                // the step's own: bits of the mask (c0: node of the word's first key)
+                const int c0 = k0 - rq.len, cn = rq.keys - rq.len;
+                if (c0 > -32 && c0 < cn) {
+                  uint32_t own;
+                  if (!a.mask) {
+                    const int n = j + 1 - c0;
+                    own = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+                    if (c0 < 0) own &= 0xffffffffu << -c0;
+                  } else {
+                    const unsigned* mw = a.mask + (size_t)row * a.words;
+                    if (c0 < 0) {
+                      own = mw[0] << -c0;
+                    } else {
+                      const int w = c0 >> 5;
+                      const uint32_t w0 = w < a.words ? mw[w] : 0u, w1 = w + 1 < a.words ? mw[w + 1] : 0u;
+                      own = __funnelshift_r(w0, w1, c0 & 31);
+                    }
+                  }
+                  if (cn - c0 < 32) own &= (1u << (cn - c0)) - 1u;
+                  if (a.window > 0)
+                    for (uint32_t left = own; left; left &= left - 1) {
+                      const int bit = __ffs(left) - 1;
+                      if (a.pos[rq.row0 + c0 + bit] <= pos - a.window) own &= ~(1u << bit);
+                    }
+                  see |= own;
+                }
+                if (holes) {
+#pragma unroll
+                  for (int h = 0; h < 2; h++) {
+                    const int pg = k0 / kKvPage + h, id = pg * kKvPage < rq.keys ? table[pg] : -1;
+                    if (id < 0 || id >= a.n_pages) see &= ~(0xffffu << (16 * h));
+                  }
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (!(see >> e & 1u)) s[k * 32 + e] = -INFINITY;
+            }
+            __syncwarp();
+          }
+          float top = s[0];
+#pragma unroll
+          for (int k = 1; k < KT; k++) top = fmaxf(top, s[k]);
+          top *= c;
+          // follow the maximum; O and l are rescaled only past the lag
+          float scale = 1.f;
+          if (l == 0.f) {
+            mx = fmaxf(mx, top);
+          } else if (live && top > mx + kTaLag) {
+            scale = ex2(mx - top);
+            mx = top;
+            l *= scale;
+          }
+          if (NS == 1 && u > 0 && !(ok = wait_warp(obar, no++ & 1))) break;
+          if (__any_sync(0xffffffffu, scale != 1.f)) {
+            fence_after();
+            const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0);
+#pragma unroll 1
+            for (int k = 0; k < HD / 32; k++) {
+              uint32_t v[32];
+              tm_ld32(op + k * 32, v);
+              tm_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
+              tm_st32(op + k * 32, v);
+            }
+          }
+          const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < KT; k++) {
+            s[k] = ex2(fmaf(s[k], c, off));
+            sum[k & 3] += s[k];
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+          for (int k = 0; k < KT / 32; k++) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const float p0 = s[k * 32 + 2 * e], p1 = s[k * 32 + 2 * e + 1];
+              hi[e] = pack2(p0, p1, C());
+              if constexpr (S::kSplit) {
+                __half2 h;
+                memcpy(&h, &hi[e], 4);
+                const float2 f = __half22float2(h);
+                lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
+              }
+            }
+            tm_st16(sp + k * 16, hi);
+            if constexpr (S::kSplit) tm_st16(sp + KT / 2 + k * 16, lo);
+          }
+          tm_wait_st();
+        } else if (NS == 1 && u > 0) {
+          no++;
+        }
+        if (key0 + KT > rq.len) {
+          // V rows that no row sees: keys past the end, nodes in nobody's mask
+          const int key = key0 + wt, node = key - rq.len;
+          bool dead = wt < KT && key >= rq.keys;
+          if (a.mask && wt < KT && node >= 0 && key < rq.keys) {
+            dead = true;
+            for (int r = rq.row0; r < rq.row0 + rq.T && dead; r++)
+              dead = a.pos[r] < 0 || (node >> 5) >= a.words || !(a.mask[(size_t)r * a.words + (node >> 5)] >> (node & 31) & 1u);
+          }
+          const uint32_t k = seq + (pair ? (uint32_t)tile * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt));
+          const uint32_t slot = k % NSLOT;
+          ok = wait_warp(full + 8 * slot, (k / NSLOT) & 1);
+          if (!ok) break;
+          if (dead) {
+            uint8_t* v = sm + S::kQBytes + slot * S::kSlot + wt * 128;
+#pragma unroll 1
+            for (int h = 0; h < ATOMS; h++)
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                *reinterpret_cast<uint4*>(v + h * KT * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async();
+        }
+        fence_before();
+        bar_arrive(pbar + 8 * b);
+      }
+      seq += 2 * nt;
+      if (!ok) break;
+      ok = wait_warp(dbar, runs++ & 1);
+      if (!ok) break;
+      if (NS == 1) no++;  // the last product's phase
+      fence_after();
+      const bool worked = NS == 2 ? t < nu : t == 0;
+      const bool merge = NS == 2 && run.whole && !pair && nu > 1;  // two streams of one row, joined here
+      const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0);
+      float* xb = reinterpret_cast<float*>(sm + S::kQTile);  // [32][128]: the second query tile's place is free
+      float own = 1.f, other = 0.f;
+      if (merge && t == 1) {
+        s_ml[wt] = make_float2(mx, l);
+      }
+      float* po = nullptr;
+      if (worked && !run.whole && live && wt < parts.prow) {
+        const size_t at = (((size_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * 2 + t) * parts.prow + wt;
+        po = parts.o + at * HD;
+        *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(mx, l);
+      }
+      Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD;
+      const bool write = run.whole && live && !(merge && t == 1);
+#pragma unroll 1
+      for (int k = 0; worked && k < HD / 32; k++) {
+        float v[32];
+        __syncwarp();
+        if (warp_live) {
+          tm_ld32(op + k * 32, reinterpret_cast<uint32_t*>(v));
+          tm_wait_ld();
+        }
+        if (merge) {
+          if (t == 1) {
+            if (nx > 0 && !(ok = wait_warp(xempty, (nx - 1) & 1))) break;
+#pragma unroll
+            for (int e = 0; e < 32; e++) xb[e * 128 + wt] = v[e];
+            bar_arrive(xfull);
+          } else {
+            if (!(ok = wait_warp(xfull, nx & 1))) break;
+            if (k == 0) {
+              const float2 ml = s_ml[wt];
+              const float mn = fmaxf(mx, ml.x);
+              own = l == 0.f ? 0.f : ex2(mx - mn);
+              other = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
+              l = l * own + ml.y * other;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = v[e] * own + xb[e * 128 + wt] * other;
+            bar_arrive(xempty);
+          }
+          nx++;
+        }
+        if (po) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) st4(po + k * 32 + e, v + e);
+        }
+        if (write) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (l == 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = 0.f;
+          }
+          if constexpr (S::kSplit) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] *= inv;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) st4((float*)out + k * 32 + e, v + e);
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) w[e] = pack2(v[2 * e] * inv, v[2 * e + 1] * inv, C());
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<uint4*>(out + k * 32 + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+          }
+        }
+      }
+      // the exchange's last round has been read before its place is written again
+      if (merge && t == 1 && ok) ok = wait_warp(xempty, (nx - 1) & 1);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+  if (tid == 0) parts.status[blockIdx.x] = s_fail;
+}
+
+// Merges the parts of the groups that were cut: a warp per (row, head).  A row
+// of a call in which a CTA's wait gave up becomes NaN.
+template <int HD, class Q>
+__global__ void __launch_bounds__(256) k_tree_combine(const TreeAttnArgs a, const Parts parts, int ctas) {
+  using S = Shape<HD, Q>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = blockIdx.x, group = a.heads / a.kv_heads;
+  pdl_wait();
+  if (r >= min(a.row_start[a.n], a.rows)) return;
+  bool failed = false;
+  for (int c = lane; c < ctas; c += 32) failed |= parts.status[c] != 0;
+  failed = __any_sync(0xffffffffu, failed);
+  int lo = 0, hi = a.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.row_start[mid + 1] > r) hi = mid;
+    else lo = mid + 1;
+  }
+  const Req q = request<S::KT>(a, lo);
+  const long long total = parts.start[a.n], base = parts.start[lo], per = (long long)q.qt * q.kt;
+  for (int head = warp; head < a.heads; head += 8) {
+    const int kvh = head / group, m = (r - q.row0) * group + head - kvh * group;
+    const int qt0 = m / 128 / S::NS * S::NS, w = min(S::NS, q.qt - qt0), wt = m & 127;
+    const long long g0 = base + kvh * per + (long long)qt0 * q.kt, g1 = g0 + (long long)w * q.kt;
+    float M = -INFINITY, L = 0.f, o[HD / 32];
+#pragma unroll
+    for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
+    bool direct = false;
+    for (long long x = g0; x < g1;) {
+      // the CTA c whose share [total c / ctas, total (c + 1) / ctas) holds x
+      const int c = (int)(((x + 1) * ctas - 1) / total);
+      const long long c0 = total * c / ctas, c1 = total * (c + 1) / ctas;
+      const long long s = max(c0, g0), e1 = min(c1, g1);
+      const int ta = (int)((s - g0) / w), tb = (int)((e1 - g0) / w);
+      x = e1;
+      if (tb <= ta) continue;
+      const int nu = w == 2 ? 2 * (tb - ta) : tb - ta;
+      if (ta == 0 && tb == q.kt) {
+        direct = true;
+        break;
+      }
+      for (int t = 0; t < S::NS; t++) {
+        if (w == 2 ? t != (m / 128 - qt0) : t >= nu) continue;
+        const size_t at = (((size_t)c * 2 + (c0 >= g0 ? 0 : 1)) * 2 + t) * parts.prow + wt;
+        const float2 ml = *reinterpret_cast<const float2*>(parts.ml + at * 2);
+        if (ml.y == 0.f) continue;
+        const float mn = fmaxf(M, ml.x), f = ex2(M - mn), g = ex2(ml.x - mn);
+        const float fo = M == -INFINITY ? 0.f : f;
+        L = L * fo + ml.y * g;
+#pragma unroll
+        for (int e = 0; e < HD / 32; e++) o[e] = o[e] * fo + parts.o[at * HD + e * 32 + lane] * g;
+        M = mn;
+      }
+    }
+    Q* out = (Q*)a.out + ((size_t)r * a.heads + head) * HD;
+    if (failed) {
+#pragma unroll
+      for (int e = 0; e < HD / 32; e++) put(out + e * 32 + lane, NAN);
+    } else if (!direct) {
+#pragma unroll
+      for (int e = 0; e < HD / 32; e++) put(out + e * 32 + lane, L == 0.f ? 0.f : o[e] / L);
+    }
+  }
+}
+
+int device_sms() {
+  static int cache[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& n = cache[dev & 63];
+  if (!n && (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)) n = 148;
+  return n;
+}
+
+// the cache as rows of head_dim values, 16 rows of 64 columns a box
+int cache_map(CUtensorMap* map, const void* base, bool bf16, int hd, size_t rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return (Encode)f;
+  }();
+  if (!encode) return fail(WL_ERR_CUDA, "tree_attention: the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)kKvPage}, step[2] = {1, 1};
+  const CUresult e = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                            const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (e != CUDA_SUCCESS) return fail(WL_ERR_CUDA, "tree_attention: tensor map refused (" + std::to_string((int)e) + ")");
+  return WL_OK;
+}
+
+template <int HD, class Q>
+int launch_t(const TreeAttnArgs& a, cudaStream_t st) {
+  using S = Shape<HD, Q>;
+  CUtensorMap mk, mv;
+  const size_t rows = (size_t)a.n_pages * a.kv_heads * kKvPage;
+  WL_TRY(cache_map(&mk, a.cache_k, S::kBf16, HD, rows));
+  WL_TRY(cache_map(&mv, a.cache_v, S::kBf16, HD, rows));
+  const int ctas = device_sms();
+  const Parts parts = parts_at(a.workspace, ctas, a.n, HD, part_rows(a.rows, a.heads / a.kv_heads));
+  constexpr int smem = kTaSmem + 1024;
+  if (first_use_on_device((const void*)k_tree_attn<HD, Q>))
+    WL_CUDA_TRY(cudaFuncSetAttribute(k_tree_attn<HD, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  WL_TRY(launch_k(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
+  return launch_k(k_tree_combine<HD, Q>, dim3(a.rows), dim3(256), 0, st, a, parts, ctas);
+}
+
+template <class Q, class C>
+int launch_hd(const TreeAttnArgs& a, cudaStream_t st) {
+  switch (a.head_dim) {
+    case 64: return launch_t<64, Q>(a, st);
+    case 128: return launch_t<128, Q>(a, st);
+    case 256: return launch_t<256, Q>(a, st);
+  }
+  return launch_k(k_tree_attn_row<Q, C>, dim3(a.rows, a.heads), dim3(128), 0, st, a);
+}
+
 }  // namespace
 
-size_t tree_attention_workspace(int, int, int, int, int, int) { return 0; }
+size_t tree_attention_workspace(int q_type, int n, int rows, int heads, int kv_heads, int head_dim) {
+  (void)q_type;
+  if (head_dim == 32) return 0;
+  return part_bytes(device_sms(), n, head_dim, part_rows(rows, heads / kv_heads));
+}
 
 int launch_tree_attention(const TreeAttnArgs& a, cudaStream_t st) {
-  const dim3 grid(a.rows, a.heads);
-  if (a.q_type == WL_F32) return launch_k(k_tree_attn_row<float, __half>, grid, dim3(128), 0, st, a);
-  if (a.q_type == WL_F16) return launch_k(k_tree_attn_row<__half, __half>, grid, dim3(128), 0, st, a);
-  return launch_k(k_tree_attn_row<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, st, a);
+  if (a.q_type == WL_F32) return launch_hd<float, __half>(a, st);
+  if (a.q_type == WL_F16) return launch_hd<__half, __half>(a, st);
+  return launch_hd<__nv_bfloat16, __nv_bfloat16>(a, st);
 }
 
 }  // namespace wl

@@ -6,6 +6,7 @@ a kernel of libwoolly_cuda.so and raises if the library or the GPU is missing.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 import numpy as np
@@ -235,42 +236,70 @@ def sample_params(rows, temperature, top_k, top_p, u) -> "np.ndarray":
 
 
 # ---------------------------------------------------------------- a serving step on a paged cache
+# These calls sit between small kernels of a decode step, where the host's time
+# per call counts: the checks below read each tensor's attributes once.
 KV_PAGE = 16  # tokens per page of a KV cache [pages, kv_heads, KV_PAGE, head_dim]
 _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_I32 = torch.int32
 
 
-def _arg(t, name, dtype=None, shape=None, device=None, rows=False) -> torch.Tensor:
-    """A CUDA tensor of the given type, shape (None: any size) and device;
-    `rows`: the first dimension may be strided."""
+def _refuse(t, name, dtype, shape, index, contiguous=True):
+    """Says what is wrong with an argument that failed its check."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype not in dtype:
+        raise ValueError(f"{name} must be {' or '.join(map(str, dtype))}, got {t.dtype}")
+    if index is not None and t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
     if shape is not None and (t.dim() != len(shape)
                               or any(w is not None and s != w for s, w in zip(t.shape, shape))):
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        if not (rows and t.dim() >= 1 and t.shape[0] > 0 and t[0].is_contiguous() and
-                t.stride(0) >= t[0].numel()):
-            raise ValueError(f"{name} must be contiguous" + (" within its rows" if rows else ""))
-    return t
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must be contiguous" + ("" if contiguous else " within its rows"))
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _i32(t, name, shape, index) -> int:
+    """Address of a contiguous int32 tensor of this shape on this device."""
+    try:
+        if t.dtype is _I32 and t.shape == shape and t.get_device() == index and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, name, (_I32,), shape, index)
 
 
-def _ld(t) -> int:
-    """Elements from one row to the next."""
-    width = t[0].numel() if t.shape[0] else t.numel()
-    return t.stride(0) if t.shape[0] > 1 else width
+def _list32(t, name, index) -> int:
+    """The same for one dimension of any size."""
+    try:
+        if t.dtype is _I32 and t.dim() == 1 and t.get_device() == index and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, name, (_I32,), (None,), index)
 
 
-def _on(t):
-    """The tensor's device as the current one, so that its current stream is used."""
-    return torch.cuda.device(t.device)
+def _row_stride(t, name, width) -> int:
+    """Elements from one row (of `width` elements, contiguous) to the next."""
+    if t.is_contiguous():
+        return width
+    st, n = t.stride(), 1
+    for size, step in zip(t.shape[:0:-1], st[:0:-1]):
+        if size != 1 and step != n:
+            _refuse(t, name, None, None, None, False)
+        n *= size
+    if t.shape[0] <= 1:
+        return width
+    if st[0] < width:
+        _refuse(t, name, None, None, None, False)
+    return st[0]
+
+
+def _launch(fn, index, *args):
+    """fn(*args, stream) on the device's current stream."""
+    if torch._C._cuda_getDevice() == index:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 class StepPlan(NamedTuple):
@@ -296,15 +325,25 @@ class Released(NamedTuple):
 
 def step_plan(n: int, rows: int, words: int = 0, device="cuda") -> StepPlan:
     """Buffers for block_tables' `out`: n requests, `rows` rows, masks of `words` words."""
-    def new(*shape):
-        return torch.empty(*shape, dtype=torch.int32, device=device)
-    return StepPlan(new(n + 1), new(rows), new(rows), new(rows), new(n), new(n), new(1), new(n + 1),
-                    new(rows, words) if words else None)
+    # one allocation; the row arrays come first
+    b = torch.empty(3 * rows + 4 * n + 3, dtype=_I32, device=device)
+    req, pos, slot, lengths, status, start, pages, free = b.split_with_sizes(
+        (rows, rows, rows, n, n, n + 1, n + 1, 1))
+    return StepPlan(start, req, pos, slot, lengths, status, free, pages,
+                    torch.empty((rows, words), dtype=_I32, device=device) if words else None)
 
 
-def _tables(tables, n=None, device=None):
-    _arg(tables, "tables", torch.int32, (n, None), device, rows=True)
-    return tables.shape[0], tables.shape[1], max(_ld(tables), tables.shape[1]), tables.device
+def _tables(tables, n, index):
+    """Device, requests, pages per row, row stride and address of a block table."""
+    try:
+        if tables.dtype is _I32 and tables.dim() == 2 and tables.is_cuda:
+            rows, pages = tables.shape
+            i = tables.get_device()
+            if (n is None or n == rows) and (index is None or index == i):
+                return i, rows, pages, _row_stride(tables, "tables", pages), tables.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(tables, "tables", (_I32,), (n, None), index)
 
 
 def block_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
@@ -324,27 +363,21 @@ def block_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tens
     plan's `positions` then count depths and its `mask` holds each row's path.
     `out` (step_plan) reuses buffers; its lengths and free_count may be the
     arguments themselves."""
-    n, pages, ld, dev = _tables(tables)
-    i32 = torch.int32
-    _arg(lengths, "lengths", i32, (n,), dev)
-    _arg(counts, "counts", i32, (n,), dev)
-    _arg(free_pages, "free_pages", i32, (None,), dev)
-    _arg(free_count, "free_count", i32, (1,), dev)
-    if parents is not None:
-        _arg(parents, "parents", i32, (rows,), dev)
+    index, n, pages, ld, at = _tables(tables, None, None)
+    each, one = (n,), (1,)
+    par = None if parents is None else _i32(parents, "parents", (rows,), index)
     if out is None:
-        out = step_plan(n, rows, words, dev)
+        out = step_plan(n, rows, words, tables.device)
     else:
-        shapes = ((n + 1,), (rows,), (rows,), (rows,), (n,), (n,), (1,), (n + 1,))
+        shapes = ((n + 1,), (rows,), (rows,), (rows,), each, each, one, (n + 1,))
         for f, t, shape in zip(StepPlan._fields, out, shapes):
-            _arg(t, f"out.{f}", i32, shape, dev)
+            _i32(t, f"out.{f}", shape, index)
         if words:
-            _arg(out.mask, "out.mask", i32, (rows, words), dev)
-    c = _lib.StepPlan(*[_ptr(t) for t in out])
-    with _on(tables):
-        check(lib().wl_block_tables(tables.data_ptr(), ld, pages, lengths.data_ptr(), counts.data_ptr(), n,
-                                    free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), rows,
-                                    _ptr(parents), words, C.byref(c), _stream()))
+            _i32(out.mask, "out.mask", (rows, words), index)
+    o = _lib.StepPlan(*[t if t is None else t.data_ptr() for t in out])
+    _launch(lib().wl_block_tables, index, at, ld, pages, _i32(lengths, "lengths", each, index),
+            _i32(counts, "counts", each, index), n, _list32(free_pages, "free_pages", index),
+            free_pages.numel(), _i32(free_count, "free_count", one, index), rows, par, words, C.byref(o))
     return out
 
 
@@ -355,29 +388,37 @@ def release_pages(tables: torch.Tensor, lengths: torch.Tensor, keep: torch.Tenso
     them go back to the stack, their table entries become -1
     (wl_release_pages).  Releasing what a step took leaves the stack as it was.
     `out`'s lengths and free_count may be the arguments themselves."""
-    n, pages, ld, dev = _tables(tables)
-    i32 = torch.int32
-    _arg(lengths, "lengths", i32, (n,), dev)
-    _arg(keep, "keep", i32, (n,), dev)
-    _arg(free_pages, "free_pages", i32, (None,), dev)
-    _arg(free_count, "free_count", i32, (1,), dev)
+    index, n, pages, ld, at = _tables(tables, None, None)
+    each, one = (n,), (1,)
     if out is None:
-        out = Released(*[torch.empty(s, dtype=i32, device=dev) for s in (n, n, 1, n + 1)])
+        b = torch.empty(3 * n + 2, dtype=_I32, device=tables.device)
+        out = Released(*b.split_with_sizes((n, n, 1, n + 1)))
     else:
-        for f, t, s in zip(Released._fields, out, (n, n, 1, n + 1)):
-            _arg(t, f"out.{f}", i32, (s,), dev)
-    c = _lib.ReleaseResult(*[_ptr(t) for t in out])
-    with _on(tables):
-        check(lib().wl_release_pages(tables.data_ptr(), ld, pages, lengths.data_ptr(), keep.data_ptr(), n,
-                                     free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-                                     C.byref(c), _stream()))
+        for f, t, shape in zip(Released._fields, out, (each, each, one, (n + 1,))):
+            _i32(t, f"out.{f}", shape, index)
+    o = _lib.ReleaseResult(*[t.data_ptr() for t in out])
+    _launch(lib().wl_release_pages, index, at, ld, pages, _i32(lengths, "lengths", each, index),
+            _i32(keep, "keep", each, index), n, _list32(free_pages, "free_pages", index),
+            free_pages.numel(), _i32(free_count, "free_count", one, index), C.byref(o))
     return out
 
 
-def _caches(cache_k, cache_v):
-    _arg(cache_k, "cache_k", (torch.float16, torch.bfloat16), (None, None, KV_PAGE, None))
-    _arg(cache_v, "cache_v", cache_k.dtype, tuple(cache_k.shape), cache_k.device)
-    return cache_k.shape[0], cache_k.shape[1], cache_k.shape[3], cache_k.device
+def _caches(k, v):
+    """Device, pages, KV heads, head_dim and type of a pair of caches."""
+    try:
+        if (k.dtype in (torch.float16, torch.bfloat16) and v.dtype is k.dtype and k.dim() == 4
+                and k.is_cuda and k.is_contiguous() and v.is_contiguous() and v.shape == k.shape
+                and v.get_device() == k.get_device()):
+            pages, kvh, page, hd = k.shape
+            if page == KV_PAGE:
+                return k.get_device(), pages, kvh, hd, k.dtype
+    except AttributeError:
+        pass
+    for t, name in ((k, "cache_k"), (v, "cache_v")):
+        if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 4 or t.shape[2] != KV_PAGE
+                or t.dtype not in (torch.float16, torch.bfloat16) or not t.is_contiguous()):
+            _refuse(t, name, (torch.float16, torch.bfloat16), (None, None, KV_PAGE, None), None)
+    _refuse(v, "cache_v", (k.dtype,), tuple(k.shape), k.get_device())
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache_k: torch.Tensor,
@@ -387,15 +428,21 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache_k: to
     rounded to the cache's f16 or bf16; f16 and bf16 rows go into a cache of
     their type.  Rows may be strided (a slice of a fused projection); slots
     outside the cache, -1 among them, are skipped; slots are distinct."""
-    pages, kvh, hd, dev = _caches(cache_k, cache_v)
-    _arg(k, "k", tuple(_TYPES), (None, kvh, hd), dev, rows=True)
-    _arg(v, "v", k.dtype, tuple(k.shape), dev, rows=True)
-    rows = k.shape[0]
-    _arg(slots, "slots", torch.int32, (rows,), dev)
-    with _on(cache_k):
-        check(lib().wl_kv_append(_TYPES[k.dtype], _TYPES[cache_k.dtype], k.data_ptr(), v.data_ptr(),
-                                 max(_ld(k), kvh * hd), max(_ld(v), kvh * hd), slots.data_ptr(), rows, kvh,
-                                 hd, pages, cache_k.data_ptr(), cache_v.data_ptr(), _stream()))
+    index, pages, kvh, hd, ct = _caches(cache_k, cache_v)
+    try:
+        st = _TYPES.get(k.dtype)
+        rows = k.shape[0]
+        shape = (rows, kvh, hd)
+        if st is None or k.shape != shape or k.get_device() != index:
+            _refuse(k, "k", tuple(_TYPES), (None, kvh, hd), index)
+        if v.dtype is not k.dtype or v.shape != shape or v.get_device() != index:
+            _refuse(v, "v", (k.dtype,), shape, index)
+    except (AttributeError, IndexError):
+        raise ValueError(f"k and v must be CUDA tensors [rows, {kvh}, {hd}]") from None
+    width = kvh * hd
+    _launch(lib().wl_kv_append, index, st, _TYPES[ct], k.data_ptr(), v.data_ptr(),
+            _row_stride(k, "k", width), _row_stride(v, "v", width), _i32(slots, "slots", (rows,), index),
+            rows, kvh, hd, pages, cache_k.data_ptr(), cache_v.data_ptr())
 
 
 def kv_commit(tables: torch.Tensor, lengths: torch.Tensor, accepted: torch.Tensor,
@@ -404,15 +451,17 @@ def kv_commit(tables: torch.Tensor, lengths: torch.Tensor, accepted: torch.Tenso
     of request i, start = accepted_start[i], goes from token lengths[i] + node
     to token lengths[i] + j.  A request's nodes are given in rising order;
     `lengths` are those before the drafts."""
-    pages, kvh, hd, dev = _caches(cache_k, cache_v)
-    n, max_pages, ld, _ = _tables(tables, device=dev)
-    _arg(lengths, "lengths", torch.int32, (n,), dev)
-    _arg(accepted, "accepted", torch.int32, (None,), dev)
-    _arg(accepted_start, "accepted_start", torch.int32, (n + 1,), dev)
-    with _on(cache_k):
-        check(lib().wl_kv_commit(_TYPES[cache_k.dtype], tables.data_ptr(), ld, max_pages, lengths.data_ptr(),
-                                 n, accepted.data_ptr(), accepted_start.data_ptr(), accepted.numel(), kvh, hd,
-                                 pages, cache_k.data_ptr(), cache_v.data_ptr(), _stream()))
+    index, pages, kvh, hd, ct = _caches(cache_k, cache_v)
+    _, n, max_pages, ld, at = _tables(tables, None, index)
+    _launch(lib().wl_kv_commit, index, _TYPES[ct], at, ld, max_pages, _i32(lengths, "lengths", (n,), index),
+            n, _list32(accepted, "accepted", index), _i32(accepted_start, "accepted_start", (n + 1,), index),
+            accepted.numel(), kvh, hd, pages, cache_k.data_ptr(), cache_v.data_ptr())
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(index, *sizes) -> int:
+    with torch.cuda.device(index):
+        return lib().wl_tree_attention_workspace(*sizes)
 
 
 def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tables: torch.Tensor,
@@ -428,39 +477,41 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     tokens and the tokens of the step that its mask bits name (block_tables'
     mask); without a mask, the step's earlier tokens and itself, so that one
     row per request is a plain decode step.  `window` > 0 keeps keys at
-    positions > positions[r] - window; `scale` defaults to head_dim ** -0.5.
+    positions > positions[r] - window (positions count from lengths[i] on);
+    `scale` defaults to head_dim ** -0.5.
     A row with a negative position or nothing to attend gives zeros; rows
     behind row_start[n] are not written.  q is f32 over an f16 cache, or has
     the cache's type; head_dim 32, 64, 128 or 256."""
-    pages, kvh, hd, dev = _caches(cache_k, cache_v)
-    _arg(q, "q", tuple(_TYPES), (None, None, hd), dev, rows=True)
-    rows, heads = q.shape[0], q.shape[1]
-    if q.dtype != cache_k.dtype and not (q.dtype == torch.float32 and cache_k.dtype == torch.float16):
-        raise ValueError(f"q must be float32 over a float16 cache or have the cache's type, got {q.dtype} "
-                         f"over {cache_k.dtype}")
-    n, max_pages, ld, _ = _tables(tables, device=dev)
-    i32 = torch.int32
-    _arg(lengths, "lengths", i32, (n,), dev)
-    _arg(row_start, "row_start", i32, (n + 1,), dev)
-    _arg(positions, "positions", i32, (rows,), dev)
-    words = 0
+    index, pages, kvh, hd, ct = _caches(cache_k, cache_v)
+    try:
+        qt = q.dtype
+        rows, heads, width = q.shape
+        if width != hd or q.get_device() != index:
+            _refuse(q, "q", None, (None, None, hd), index)
+    except (AttributeError, ValueError):
+        _refuse(q, "q", None, (None, None, hd), index)
+    if qt is not ct and not (qt is torch.float32 and ct is torch.float16):
+        raise ValueError(f"q must be float32 over a float16 cache or have the cache's type, got {qt} over {ct}")
+    _, n, max_pages, ld, at = _tables(tables, None, index)
+    words = m = None
     if mask is not None:
-        _arg(mask, "mask", i32, (rows, None), dev)
-        words = mask.shape[1]
+        try:
+            words = mask.shape[1]
+        except (AttributeError, IndexError):
+            _refuse(mask, "mask", (_I32,), (rows, None), index)
+        m = _i32(mask, "mask", (rows, words), index)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _arg(out, "out", q.dtype, tuple(q.shape), dev)
-    qt = _TYPES[q.dtype]
-    with _on(q):
-        nb = lib().wl_tree_attention_workspace(qt, n, rows, heads, kvh, hd)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        check(lib().wl_tree_attention(qt, q.data_ptr(), max(_ld(q), heads * hd), cache_k.data_ptr(),
-                                      cache_v.data_ptr(), pages, tables.data_ptr(), ld, max_pages,
-                                      lengths.data_ptr(), row_start.data_ptr(), positions.data_ptr(),
-                                      _ptr(mask), words, n, rows, heads, kvh, hd, int(window),
-                                      hd ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                                      _ptr(ws), nb, _stream()))
+        out = torch.empty(q.shape, dtype=qt, device=q.device)
+    elif out.dtype is not qt or out.shape != q.shape or out.get_device() != index or not out.is_contiguous():
+        _refuse(out, "out", (qt,), tuple(q.shape), index)
+    t = _TYPES[qt]
+    nb = _attention_workspace(index, t, n, rows, heads, kvh, hd)
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+    _launch(lib().wl_tree_attention, index, t, q.data_ptr(), _row_stride(q, "q", heads * hd),
+            cache_k.data_ptr(), cache_v.data_ptr(), pages, at, ld, max_pages,
+            _i32(lengths, "lengths", (n,), index), _i32(row_start, "row_start", (n + 1,), index),
+            _i32(positions, "positions", (rows,), index), m, words or 0, n, rows, heads, kvh, hd,
+            int(window), hd ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), nb)
     return out
 
 
@@ -497,52 +548,64 @@ def process_logits(logits: torch.Tensor, params: torch.Tensor, *, history: torch
     allowed [masks, words]: bit v % 32 of word v // 32 set means token v may
     follow; params' allowed_row picks the mask of each row.  Integers are
     int32.  `out` may be `logits`."""
-    _arg(logits, "logits", tuple(_TYPES), (None, None), rows=True)
-    rows, V = logits.shape
-    dev, i32 = logits.device, torch.int32
-    _arg(params, "params", torch.uint8, (None,), dev)
+    try:
+        lt = _TYPES.get(logits.dtype)
+        rows, V = logits.shape
+        index = logits.get_device()
+        if lt is None or index < 0:
+            _refuse(logits, "logits", tuple(_TYPES), (None, None), None)
+    except (AttributeError, ValueError):
+        _refuse(logits, "logits", tuple(_TYPES), (None, None), None)
+    if (params.dtype is not torch.uint8 or params.get_device() != index or not params.is_contiguous()):
+        _refuse(params, "params", (torch.uint8,), (None,), index)
     if params.numel() < rows * 16:
         raise ValueError(f"params must hold {rows} records")
     c = _lib.LogitContext()
-    n = None
+    n, every = 0, (rows,)
     if history_start is not None or history is not None:
-        _arg(history_start, "history_start", i32, (None,), dev)
-        _arg(history, "history", i32, (None,), dev)
+        c.history_start = _list32(history_start, "history_start", index)
+        c.history = _list32(history, "history", index)
+        c.history_total = history.numel()
         n = history_start.numel() - 1
         if n < 0:
             raise ValueError("history_start must have one entry more than there are requests")
-        c.history, c.history_start, c.history_total = history.data_ptr(), history_start.data_ptr(), history.numel()
     if prompt_lens is not None:
-        if n is None:
+        if history is None:
             raise ValueError("prompt_lens needs a history")
-        c.prompt_lens = _arg(prompt_lens, "prompt_lens", i32, (n,), dev).data_ptr()
+        c.prompt_lens = _i32(prompt_lens, "prompt_lens", (n,), index)
     if draft_mask is not None or draft_tokens is not None:
-        _arg(draft_mask, "draft_mask", i32, (rows, None), dev)
-        _arg(draft_tokens, "draft_tokens", i32, (rows,), dev)
-        _arg(row_start, "row_start", i32, (None if n is None else n + 1,), dev)
+        if draft_mask is None or draft_tokens is None or row_start is None:
+            raise ValueError("drafts need draft_tokens, draft_mask and row_start")
+        c.words = draft_mask.shape[1] if draft_mask.dim() == 2 else 0
+        c.draft_mask = _i32(draft_mask, "draft_mask", (rows, c.words), index)
+        c.draft_tokens = _i32(draft_tokens, "draft_tokens", every, index)
+        c.row_start = _list32(row_start, "row_start", index)
+        if history is not None and row_start.numel() != n + 1:
+            raise ValueError(f"row_start must have {n + 1} entries, got {row_start.numel()}")
         n = row_start.numel() - 1
-        c.draft_mask, c.words = draft_mask.data_ptr(), draft_mask.shape[1]
-        c.draft_tokens, c.row_start = draft_tokens.data_ptr(), row_start.data_ptr()
-    c.n_history = n or 0
+    c.n_history = n
     if requests is not None:
-        c.requests = _arg(requests, "requests", i32, (rows,), dev).data_ptr()
+        c.requests = _i32(requests, "requests", every, index)
     if bias_start is not None or bias_tokens is not None or bias_values is not None:
-        _arg(bias_start, "bias_start", i32, (rows + 1,), dev)
-        _arg(bias_tokens, "bias_tokens", i32, (None,), dev)
-        _arg(bias_values, "bias_values", torch.float32, (bias_tokens.numel(),), dev)
-        c.bias_start, c.bias_tokens = bias_start.data_ptr(), bias_tokens.data_ptr()
-        c.bias_values, c.bias_total = bias_values.data_ptr(), bias_tokens.numel()
+        c.bias_start = _i32(bias_start, "bias_start", (rows + 1,), index)
+        c.bias_tokens = _list32(bias_tokens, "bias_tokens", index)
+        c.bias_total = nb = bias_tokens.numel()
+        if (bias_values is None or bias_values.dtype is not torch.float32 or bias_values.shape != (nb,)
+                or bias_values.get_device() != index or not bias_values.is_contiguous()):
+            _refuse(bias_values, "bias_values", (torch.float32,), (nb,), index)
+        c.bias_values = bias_values.data_ptr()
     if allowed is not None:
-        _arg(allowed, "allowed", i32, (None, None), dev)
-        c.allowed, c.n_allowed, c.allowed_words = allowed.data_ptr(), allowed.shape[0], allowed.shape[1]
+        try:
+            c.n_allowed, c.allowed_words = allowed.shape
+        except (AttributeError, ValueError):
+            _refuse(allowed, "allowed", (_I32,), (None, None), index)
+        c.allowed = _i32(allowed, "allowed", (c.n_allowed, c.allowed_words), index)
     if out is None:
-        out = torch.empty((rows, V), dtype=logits.dtype, device=dev)
-    else:
-        _arg(out, "out", logits.dtype, (rows, V), dev, rows=True)
-    with _on(logits):
-        check(lib().wl_process_logits(_TYPES[logits.dtype], logits.data_ptr(), max(_ld(logits), V), rows, V,
-                                      params.data_ptr(), C.byref(c), out.data_ptr(), max(_ld(out), V),
-                                      _stream()))
+        out = torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
+    elif out.dtype is not logits.dtype or out.shape != (rows, V) or out.get_device() != index:
+        _refuse(out, "out", (logits.dtype,), (rows, V), index, False)
+    _launch(lib().wl_process_logits, index, lt, logits.data_ptr(), _row_stride(logits, "logits", V), rows, V,
+            params.data_ptr(), C.byref(c), out.data_ptr(), _row_stride(out, "out", V))
     return out
 
 
