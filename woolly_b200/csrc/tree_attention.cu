@@ -227,7 +227,11 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t* v) {
       WL_I8(v, 8), "r"(a)
       : "memory");
 }
-__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+// the loads into v have arrived: v passes through, so that no use moves before the wait
+#define WL_P8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+__device__ __forceinline__ void tm_wait_ld(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : WL_P8(v, 0), WL_P8(v, 8), WL_P8(v, 16), WL_P8(v, 24)::"memory");
+}
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -272,6 +276,19 @@ __device__ __forceinline__ long long units(const TreeAttnArgs& a, const Req& q) 
   return (long long)a.kv_heads * q.qt * q.kt;
 }
 
+// Mask bits of nodes c0 .. c0 + 31 of a row (c0 > -32; nodes below 0: clear).
+__device__ __forceinline__ uint32_t mask_bits(const TreeAttnArgs& a, int row, int c0) {
+  const unsigned* m = a.mask + (size_t)row * a.words;
+  if (c0 < 0) return m[0] << -c0;
+  const int w = c0 >> 5;
+  const uint32_t w0 = w < a.words ? m[w] : 0u, w1 = w + 1 < a.words ? m[w + 1] : 0u;
+  return __funnelshift_r(w0, w1, c0 & 31);
+}
+
+__device__ __forceinline__ long long quot(long long a, long long b) {  // a >= 0, b > 0
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // A run of key tiles [a, b) of one group: KV head kvh, query tiles qt0 .. qt0 + w - 1
 struct Run {
   int i, kvh, qt0, w, a, b;
@@ -293,15 +310,15 @@ struct Walk {
       }
       const long long per = (long long)q.qt * q.kt;
       const long long off = x - base;
-      r.kvh = (int)(off / per);
+      r.kvh = (int)quot(off, per);
       const long long y = off - r.kvh * per;
-      r.qt0 = (int)(y / ((long long)S::NS * q.kt)) * S::NS;
+      r.qt0 = (int)quot(y, (long long)S::NS * q.kt) * S::NS;
       r.w = min(S::NS, q.qt - r.qt0);
       const long long g0 = base + r.kvh * per + (long long)r.qt0 * q.kt;
       const long long g1 = g0 + (long long)r.w * q.kt, e = min(x1, g1);
       r.i = i;
-      r.a = (int)((x - g0) / r.w);
-      r.b = (int)((e - g0) / r.w);
+      r.a = (int)((x - g0) >> (r.w - 1));  // w is 1 or 2
+      r.b = (int)((e - g0) >> (r.w - 1));
       r.first = x0 >= g0;
       r.whole = r.a == 0 && r.b == q.kt;
       x = e;
@@ -315,7 +332,7 @@ struct Walk {
 // each; one status word per CTA and the requests' prefix sums before them.
 struct Parts {
   int* status;       // [ctas]
-  long long* start;  // [n + 1]
+  long long* start;  // [n] prefix sums, then the total and a CTA's share
   float* o;
   float* ml;
   int prow;          // rows kept of a 128-row tile
@@ -326,14 +343,14 @@ __host__ inline int part_rows(int rows, int group) {
   return m < 128 ? (int)m : 128;
 }
 __host__ inline size_t part_bytes(int ctas, int n, int hd, int prow) {
-  return round256((size_t)ctas * 4) + round256((size_t)(n + 1) * 8) + (size_t)ctas * 4 * prow * (hd + 2) * 4;
+  return round256((size_t)ctas * 4) + round256((size_t)(n + 2) * 8) + (size_t)ctas * 4 * prow * (hd + 2) * 4;
 }
 __host__ inline Parts parts_at(void* ws, int ctas, int n, int hd, int prow) {
   Parts p;
   uint8_t* b = (uint8_t*)ws;
   p.status = (int*)b;
   p.start = (long long*)(b + round256((size_t)ctas * 4));
-  p.o = (float*)(b + round256((size_t)ctas * 4) + round256((size_t)(n + 1) * 8));
+  p.o = (float*)(b + round256((size_t)ctas * 4) + round256((size_t)(n + 2) * 8));
   p.ml = p.o + (size_t)ctas * 4 * prow * hd;
   p.prow = prow;
   return p;
@@ -355,6 +372,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   __shared__ int s_fail;
   __shared__ long long s_scan[kTaThreads / 32], s_base;
   __shared__ int s_req;
+  __shared__ Req s_q;
   __shared__ float2 s_ml[128];
   const uint32_t full = sptr(s_bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
                  pbar = sbar + 16, dbar = pbar + 16, obar = dbar + 8, endbar = obar + 8, xfull = endbar + 8, xempty = xfull + 8;
@@ -404,22 +422,31 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       before = w + x - v;
       return all;
     };
-    long long total = 0, before;
-    for (int i0 = 0; i0 < a.n; i0 += kTaThreads)
-      total += block_sum(i0 + tid < a.n ? units(a, request<KT>(a, i0 + tid)) : 0, before);
-    walk.x0 = walk.x = total * blockIdx.x / gridDim.x;
-    walk.x1 = total * (blockIdx.x + 1) / gridDim.x;
+    long long total = 0, before, u = 0;
+    Req q{};
+    for (int i0 = 0; i0 < a.n; i0 += kTaThreads) {
+      if (i0 + tid < a.n) q = request<KT>(a, i0 + tid);
+      u = i0 + tid < a.n ? units(a, q) : 0;
+      total += block_sum(u, before);
+    }
+    const long long per = total > 0 ? quot(total + gridDim.x - 1, gridDim.x) : 1;
+    walk.x0 = walk.x = min(total, per * blockIdx.x);
+    walk.x1 = min(total, walk.x0 + per);
     long long sum = 0;
     for (int i0 = 0; i0 < a.n; i0 += kTaThreads) {
       const int i = i0 + tid;
-      const long long u = i < a.n ? units(a, request<KT>(a, i)) : 0;
-      const long long all = block_sum(u, before);
+      long long all = total;
+      if (a.n > kTaThreads) {  // otherwise the sums above stand
+        if (i < a.n) q = request<KT>(a, i);
+        u = i < a.n ? units(a, q) : 0;
+        all = block_sum(u, before);
+      }
       before += sum;
-      if (walk.x >= before && walk.x < before + u) s_req = i, s_base = before;
+      if (walk.x >= before && walk.x < before + u) s_req = i, s_base = before, s_q = q;
       if (blockIdx.x == 0 && i < a.n) parts.start[i] = before;
       sum += all;
     }
-    if (blockIdx.x == 0 && tid == 0) parts.start[a.n] = total;
+    if (blockIdx.x == 0 && tid == 0) parts.start[a.n] = total, parts.start[a.n + 1] = per;
   }
   fence_before();
   __syncthreads();
@@ -428,7 +455,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   if (walk.x < walk.x1) {
     walk.i = s_req;
     walk.base = s_base;
-    walk.q = request<KT>(a, walk.i);
+    walk.q = s_q;
   }
   Run run;
 
@@ -510,7 +537,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ks++) {
               const uint32_t o = (ks >> 2) * 128 * 128 + (ks & 3) * 32, ok_ = (ks >> 2) * KT * 128 + (ks & 3) * 32;
-              mma_ss(d, sw128_desc(qb + w * NS * S::kQTile + o, 16, 1024), sw128_desc(kb + ok_, 16, 1024), S::kIdescS,
+              mma_ss(d, sw128_desc(qb + (S::kSplit && !w ? NS * S::kQTile : 0) + o, 16, 1024),
+                     sw128_desc(kb + ok_, 16, 1024), S::kIdescS,
                      w || ks ? 1u : 0u);
             }
           mma_commit(sbar + 8 * (u & 1));
@@ -533,8 +561,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
 #pragma unroll
             for (int ks = 0; ks < KT / 16; ks++)
-              mma_ts(d, p + w * (KT / 2) + ks * 8, sw128_desc(vb + ks * 16 * 128, KT * 128, 1024), S::kIdescO,
-                     fresh && !w && !ks ? 0u : 1u);
+              // the low words first: sums are cut off rather than rounded, and
+              // that costs least while they are small
+              mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8 + (S::kSplit && !w ? 16 : 0),
+                     sw128_desc(vb + ks * 16 * 128, KT * 128, 1024), S::kIdescO, fresh && !w && !ks ? 0u : 1u);
           if (!pair || b) mma_commit(empty + 8 * slot);
           if (NS == 1) mma_commit(obar);
           if (u + 2 < nu) scores(u + 2);
@@ -613,6 +643,41 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         holes = __any_sync(0xffffffffu, holes);
       }
+      // bits of the keys k0 .. k0 + 31 that this thread's row attends
+      auto visible = [&](int k0) {
+        uint32_t see = 0;
+        if (pos < 0) return see;
+        // cached tokens: a range
+        const int lo = a.window > 0 ? max(pos - a.window + 1 - k0, 0) : 0, hi = min(rq.len - k0, 32);
+        if (hi > lo) see = (hi >= 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+        // the step's own: bits of the mask (c0: node of the word's first key)
+        const int c0 = k0 - rq.len, cn = rq.keys - rq.len;
+        if (c0 > -32 && c0 < cn) {
+          uint32_t own;
+          if (!a.mask) {
+            const int n = j + 1 - c0;
+            own = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+            if (c0 < 0) own &= 0xffffffffu << -c0;
+          } else {
+            own = mask_bits(a, row, c0);
+          }
+          if (cn - c0 < 32) own &= (1u << (cn - c0)) - 1u;
+          if (a.window > 0)
+            for (uint32_t left = own; left; left &= left - 1) {
+              const int bit = __ffs(left) - 1;
+              if (a.pos[rq.row0 + c0 + bit] <= pos - a.window) own &= ~(1u << bit);
+            }
+          see |= own;
+        }
+        if (holes) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int pg = k0 / kKvPage + h, id = pg * kKvPage < rq.keys ? table[pg] : -1;
+            if (id < 0 || id >= a.n_pages) see &= ~(0xffffu << (16 * h));
+          }
+        }
+        return see;
+      };
       float mx = -INFINITY, l = 0.f;
       const int step = NS == 2 ? 2 : 1;
       for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step) {
@@ -621,64 +686,31 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (!ok) break;
         fence_after();
         const uint32_t sp = tmem + lanes + b * KT;
-        float s[KT];
         if (warp_live) {
-#pragma unroll
-          for (int k = 0; k < KT / 32; k++) tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s) + k * 32);
-          tm_wait_ld();
+          // which keys the row sees, when it is not all of them
           const bool plain = key0 + KT <= rq.len && !holes && (a.window <= 0 || key0 > pos - a.window) && pos >= 0;
-          if (!__all_sync(0xffffffffu, plain || !live)) {
+          const bool masked = !__all_sync(0xffffffffu, plain || !live);
+          uint32_t see[KT / 32];
+          if (masked) {
 #pragma unroll
-            for (int k = 0; k < KT / 32; k++) {
-              const int k0 = key0 + 32 * k;
-              uint32_t see = 0;
-              if (pos >= 0) {
-                // cached tokens: a range
-                const int lo = a.window > 0 ? max(pos - a.window + 1 - k0, 0) : 0, hi = min(rq.len - k0, 32);
-                if (hi > lo) see = (hi >= 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
-                // the step's own: bits of the mask (c0: node of the word's first key)
-                const int c0 = k0 - rq.len, cn = rq.keys - rq.len;
-                if (c0 > -32 && c0 < cn) {
-                  uint32_t own;
-                  if (!a.mask) {
-                    const int n = j + 1 - c0;
-                    own = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
-                    if (c0 < 0) own &= 0xffffffffu << -c0;
-                  } else {
-                    const unsigned* mw = a.mask + (size_t)row * a.words;
-                    if (c0 < 0) {
-                      own = mw[0] << -c0;
-                    } else {
-                      const int w = c0 >> 5;
-                      const uint32_t w0 = w < a.words ? mw[w] : 0u, w1 = w + 1 < a.words ? mw[w + 1] : 0u;
-                      own = __funnelshift_r(w0, w1, c0 & 31);
-                    }
-                  }
-                  if (cn - c0 < 32) own &= (1u << (cn - c0)) - 1u;
-                  if (a.window > 0)
-                    for (uint32_t left = own; left; left &= left - 1) {
-                      const int bit = __ffs(left) - 1;
-                      if (a.pos[rq.row0 + c0 + bit] <= pos - a.window) own &= ~(1u << bit);
-                    }
-                  see |= own;
-                }
-                if (holes) {
-#pragma unroll
-                  for (int h = 0; h < 2; h++) {
-                    const int pg = k0 / kKvPage + h, id = pg * kKvPage < rq.keys ? table[pg] : -1;
-                    if (id < 0 || id >= a.n_pages) see &= ~(0xffffu << (16 * h));
-                  }
-                }
-              }
-#pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (!(see >> e & 1u)) s[k * 32 + e] = -INFINITY;
-            }
+            for (int k = 0; k < KT / 32; k++) see[k] = visible(key0 + 32 * k);
             __syncwarp();
           }
-          float top = s[0];
+          // S comes in 32 columns at a time, once for the maximum and once for P
+          float s[32], top = -INFINITY;
 #pragma unroll
-          for (int k = 1; k < KT; k++) top = fmaxf(top, s[k]);
+          for (int k = 0; k < KT / 32; k++) {
+            tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
+            tm_wait_ld(reinterpret_cast<uint32_t*>(s));
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
+            }
+            float t4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int e = 4; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], s[e]);
+            top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+          }
           top *= c;
           // follow the maximum; O and l are rescaled only past the lag
           float scale = 1.f;
@@ -695,28 +727,29 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0);
 #pragma unroll 1
             for (int k = 0; k < HD / 32; k++) {
-              uint32_t v[32];
-              tm_ld32(op + k * 32, v);
-              tm_wait_ld();
+              tm_ld32(op + k * 32, reinterpret_cast<uint32_t*>(s));
+              tm_wait_ld(reinterpret_cast<uint32_t*>(s));
 #pragma unroll
-              for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
-              tm_st32(op + k * 32, v);
+              for (int e = 0; e < 32; e++) s[e] *= scale;
+              tm_st32(op + k * 32, reinterpret_cast<uint32_t*>(s));
             }
           }
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < KT; k++) {
-            s[k] = ex2(fmaf(s[k], c, off));
-            sum[k & 3] += s[k];
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
           for (int k = 0; k < KT / 32; k++) {
+            tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
+            tm_wait_ld(reinterpret_cast<uint32_t*>(s));
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
+            }
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-              const float p0 = s[k * 32 + 2 * e], p1 = s[k * 32 + 2 * e + 1];
+              const float p0 = ex2(fmaf(s[2 * e], c, off)), p1 = ex2(fmaf(s[2 * e + 1], c, off));
+              sum[(2 * e) & 3] += p0;
+              sum[(2 * e + 1) & 3] += p1;
               hi[e] = pack2(p0, p1, C());
               if constexpr (S::kSplit) {
                 __half2 h;
@@ -725,21 +758,34 @@ __global__ void __launch_bounds__(kTaThreads, 1)
                 lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
               }
             }
-            tm_st16(sp + k * 16, hi);
-            if constexpr (S::kSplit) tm_st16(sp + KT / 2 + k * 16, lo);
+            // over the scores they came from: the high words, then the low ones
+            tm_st16(sp + k * 32, hi);
+            if constexpr (S::kSplit) tm_st16(sp + k * 32 + 16, lo);
           }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tm_wait_st();
         } else if (NS == 1 && u > 0) {
           no++;
         }
         if (key0 + KT > rq.len) {
-          // V rows that no row sees: keys past the end, nodes in nobody's mask
-          const int key = key0 + wt, node = key - rq.len;
-          bool dead = wt < KT && key >= rq.keys;
-          if (a.mask && wt < KT && node >= 0 && key < rq.keys) {
-            dead = true;
-            for (int r = rq.row0; r < rq.row0 + rq.T && dead; r++)
-              dead = a.pos[r] < 0 || (node >> 5) >= a.words || !(a.mask[(size_t)r * a.words + (node >> 5)] >> (node & 31) & 1u);
+          // V rows that no row sees: keys past the end, nodes in nobody's mask.
+          // A warp takes 32 keys, its lanes the request's rows.
+          const int k0 = key0 + (wt & ~31);
+          bool dead = false;
+          if (wt < KT) {
+            uint32_t seen = 0;
+            if (!a.mask || k0 + 32 <= rq.len) {
+              seen = 0xffffffffu;
+            } else if (k0 < rq.keys) {
+#pragma unroll 2
+              for (int r = lane; r < rq.T; r += 32) {
+                const uint32_t bits = mask_bits(a, rq.row0 + r, k0 - rq.len);
+                if (a.pos[rq.row0 + r] >= 0) seen |= bits;
+              }
+              seen = __reduce_or_sync(0xffffffffu, seen);
+              if (k0 < rq.len) seen |= (1u << (rq.len - k0)) - 1u;  // cached tokens of the word
+            }
+            dead = key0 + wt >= rq.keys || !(seen >> lane & 1u);
           }
           const uint32_t k = seq + (pair ? (uint32_t)tile * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt));
           const uint32_t slot = k % NSLOT;
@@ -786,7 +832,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         __syncwarp();
         if (warp_live) {
           tm_ld32(op + k * 32, reinterpret_cast<uint32_t*>(v));
-          tm_wait_ld();
+          tm_wait_ld(reinterpret_cast<uint32_t*>(v));
         }
         if (merge) {
           if (t == 1) {
@@ -844,15 +890,17 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   if (tid == 0) parts.status[blockIdx.x] = s_fail;
 }
 
-// Merges the parts of the groups that were cut: a warp per (row, head).  A row
-// of a call in which a CTA's wait gave up becomes NaN.
+// Merges the parts of the groups that were cut: a warp per (row, head), its
+// lanes a part each for the weights, then HD / 32 columns each.  A row of a call
+// in which a CTA's wait gave up becomes NaN.
 template <int HD, class Q>
-__global__ void __launch_bounds__(256) k_tree_combine(const TreeAttnArgs a, const Parts parts, int ctas) {
+__global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, const Parts parts, int ctas) {
   using S = Shape<HD, Q>;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = blockIdx.x, group = a.heads / a.kv_heads;
+  const int lane = threadIdx.x & 31, r = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int group = a.heads / a.kv_heads;
   pdl_wait();
-  if (r >= min(a.row_start[a.n], a.rows)) return;
+  if (head >= a.heads || r >= min(a.row_start[a.n], a.rows)) return;
+  const long long per = parts.start[a.n + 1];
   bool failed = false;
   for (int c = lane; c < ctas; c += 32) failed |= parts.status[c] != 0;
   failed = __any_sync(0xffffffffu, failed);
@@ -863,50 +911,56 @@ __global__ void __launch_bounds__(256) k_tree_combine(const TreeAttnArgs a, cons
     else lo = mid + 1;
   }
   const Req q = request<S::KT>(a, lo);
-  const long long total = parts.start[a.n], base = parts.start[lo], per = (long long)q.qt * q.kt;
-  for (int head = warp; head < a.heads; head += 8) {
-    const int kvh = head / group, m = (r - q.row0) * group + head - kvh * group;
-    const int qt0 = m / 128 / S::NS * S::NS, w = min(S::NS, q.qt - qt0), wt = m & 127;
-    const long long g0 = base + kvh * per + (long long)qt0 * q.kt, g1 = g0 + (long long)w * q.kt;
-    float M = -INFINITY, L = 0.f, o[HD / 32];
+  const int kvh = head / group, m = (r - q.row0) * group + head - kvh * group;
+  const int qt0 = m / 128 / S::NS * S::NS, w = min(S::NS, q.qt - qt0), wt = m & 127;
+  if (w < 1 || m < 0) return;
+  const long long g0 = parts.start[lo] + (long long)kvh * q.qt * q.kt + (long long)qt0 * q.kt;
+  const long long g1 = g0 + (long long)w * q.kt;
+  const int c0 = (int)quot(g0, per), c1 = (int)quot(g1 - 1, per);
+  // parts: both streams of each CTA of the group, or the query tile's own
+  const int nt = w == 2 ? 1 : S::NS, np = (c1 - c0 + 1) * nt;
+  float M = -INFINITY, L = 0.f, o[HD / 32];
 #pragma unroll
-    for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
-    bool direct = false;
-    for (long long x = g0; x < g1;) {
-      // the CTA c whose share [total c / ctas, total (c + 1) / ctas) holds x
-      const int c = (int)(((x + 1) * ctas - 1) / total);
-      const long long c0 = total * c / ctas, c1 = total * (c + 1) / ctas;
-      const long long s = max(c0, g0), e1 = min(c1, g1);
-      const int ta = (int)((s - g0) / w), tb = (int)((e1 - g0) / w);
-      x = e1;
-      if (tb <= ta) continue;
-      const int nu = w == 2 ? 2 * (tb - ta) : tb - ta;
-      if (ta == 0 && tb == q.kt) {
-        direct = true;
-        break;
-      }
-      for (int t = 0; t < S::NS; t++) {
-        if (w == 2 ? t != (m / 128 - qt0) : t >= nu) continue;
-        const size_t at = (((size_t)c * 2 + (c0 >= g0 ? 0 : 1)) * 2 + t) * parts.prow + wt;
-        const float2 ml = *reinterpret_cast<const float2*>(parts.ml + at * 2);
-        if (ml.y == 0.f) continue;
-        const float mn = fmaxf(M, ml.x), f = ex2(M - mn), g = ex2(ml.x - mn);
-        const float fo = M == -INFINITY ? 0.f : f;
-        L = L * fo + ml.y * g;
-#pragma unroll
-        for (int e = 0; e < HD / 32; e++) o[e] = o[e] * fo + parts.o[at * HD + e * 32 + lane] * g;
-        M = mn;
-      }
+  for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
+  for (int p0 = 0; p0 < np; p0 += 32) {
+    const int p = p0 + lane, c = c0 + p / nt, t = w == 2 ? m / 128 - qt0 : p % nt;
+    const long long s = max((long long)c * per, g0), e1 = min((long long)(c + 1) * per, g1);
+    const int ta = (int)((s - g0) >> (w - 1)), tb = (int)((e1 - g0) >> (w - 1));
+    const bool ok = p < np && tb > ta && (w == 2 || t < tb - ta);
+    if (__any_sync(0xffffffffu, ok && ta == 0 && tb == q.kt)) {  // one CTA had it all and wrote the row
+      if (!failed) return;
+      break;
     }
-    Q* out = (Q*)a.out + ((size_t)r * a.heads + head) * HD;
-    if (failed) {
+    const size_t at = (((size_t)c * 2 + ((long long)c * per >= g0 ? 0 : 1)) * 2 + t) * parts.prow + wt;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (ok) ml = *reinterpret_cast<const float2*>(parts.ml + at * 2);
+    float top = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
-      for (int e = 0; e < HD / 32; e++) put(out + e * 32 + lane, NAN);
-    } else if (!direct) {
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float mn = fmaxf(M, top), old = M == -INFINITY ? 0.f : ex2(M - mn);
+    const float f = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
+    float sum = ml.y * f;
+    if (ml.y == 0.f) sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < HD / 32; e++) put(out + e * 32 + lane, L == 0.f ? 0.f : o[e] / L);
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    L = L * old + sum;
+    M = mn;
+#pragma unroll
+    for (int e = 0; e < HD / 32; e++) o[e] *= old;
+    const unsigned live = __ballot_sync(0xffffffffu, ml.y != 0.f);
+#pragma unroll 4
+    for (int k = 0; k < min(32, np - p0); k++) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      const size_t ak = __shfl_sync(0xffffffffu, at, k);
+      if (live >> k & 1u) {
+#pragma unroll
+        for (int e = 0; e < HD / 32; e++) o[e] += parts.o[ak * HD + e * 32 + lane] * fk;
+      }
     }
   }
+  Q* out = (Q*)a.out + ((size_t)r * a.heads + head) * HD;
+#pragma unroll
+  for (int e = 0; e < HD / 32; e++) put(out + e * 32 + lane, failed ? NAN : L == 0.f ? 0.f : o[e] / L);
 }
 
 int device_sms() {
@@ -955,7 +1009,12 @@ int launch_t(const TreeAttnArgs& a, cudaStream_t st) {
   if (first_use_on_device((const void*)k_tree_attn<HD, Q>))
     WL_CUDA_TRY(cudaFuncSetAttribute(k_tree_attn<HD, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   WL_TRY(launch_k(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
-  return launch_k(k_tree_combine<HD, Q>, dim3(a.rows), dim3(256), 0, st, a, parts, ctas);
+  // the merge is launched under the main kernel and waits for its end
+  const bool was = pdl_enabled();
+  set_pdl(true);
+  const int e = launch_k(k_tree_combine<HD, Q>, dim3(a.rows, (a.heads + 3) / 4), dim3(128), 0, st, a, parts, ctas);
+  set_pdl(was);
+  return e;
 }
 
 template <class Q, class C>
