@@ -15,13 +15,14 @@
 // cut evenly over one CTA per SM, whatever the lengths, each CTA finding its
 // share from a prefix sum over the requests.  A run that is not a whole group
 // leaves unnormalised parts (o, m, l), which k_tree_combine merges.
-//   warp 8     brings K and V tiles in with TMA, a 16-token page at a time
+//   a warp     brings K and V tiles in with TMA, a 16-token page at a time
 //              (its 64-column halves land in 128-byte-swizzled rows);
-//   warp 9     issues S = Q K^T into TMEM and O += P V (P from TMEM, V as the
+//   a warp     issues S = Q K^T into TMEM and O += P V (P from TMEM, V as the
 //              MN-major operand straight from its rows);
-//   warps 0-7  two softmax groups, a thread per query row: S from TMEM into
-//              registers, mask, running maximum and sum, P back over S.
-// The groups work on two streams, so that one's softmax runs under the other's
+//   others     softmax, two threads per query row (half of a key tile's columns
+//              each): S from TMEM into registers, mask, running maximum and sum,
+//              P back over S.
+// They work on two streams, so that one's softmax runs under the other's
 // products: the two query tiles of a pair over the same keys or, for a single
 // query tile, even and odd key tiles, merged with the parts.  head_dim 256 has
 // room in TMEM for one O only: one stream, with S double-buffered.
@@ -132,7 +133,8 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
 
 
 // ---------------------------------------------------------------- tcgen05
-constexpr int kTaThreads = 320;
+constexpr int kTaSoft = 16;          // softmax warps: 2 streams x 2 halves of the key tile x 4 lane quarters
+constexpr int kTaThreads = (kTaSoft + 2) * 32;
 constexpr int kTaSmem = 224 * 1024;   // query tiles, then the ring of K / V tiles
 constexpr int kTaLag = 6;             // log2 of the lag of the maximum
 
@@ -177,23 +179,29 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   *failed = 1;
   return false;
 }
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
-         (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Shared-memory operands: the descriptor's low word is the address (in 16-byte
+// units, with the leading offset above it), the high word fixed for a layout
+// (stride between 8-row groups 1024 bytes, version 1, 128-byte swizzle).
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return (addr >> 4) | (lead >> 4) << 16; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
       : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
@@ -213,12 +221,16 @@ __device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t* v) {
       : WL_R8(v, 0), WL_R8(v, 8), WL_R8(v, 16), WL_R8(v, 24)
       : "r"(a));
 }
-__device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t* v) {
+__device__ __forceinline__ void tm_ld16(uint32_t a, uint32_t* v) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n" ::WL_I8(v, 0),
-      WL_I8(v, 8), WL_I8(v, 16), WL_I8(v, 24), "r"(a)
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n"
+      : WL_R8(v, 0), WL_R8(v, 8)
+      : "r"(a));
+}
+__device__ __forceinline__ void tm_st8(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};\n" ::WL_I8(v, 0), "r"(a)
+               : "memory");
 }
 __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t* v) {
   asm volatile(
@@ -231,6 +243,9 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t* v) {
 #define WL_P8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
 __device__ __forceinline__ void tm_wait_ld(uint32_t* v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" : WL_P8(v, 0), WL_P8(v, 8), WL_P8(v, 16), WL_P8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tm_wait_ld16(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : WL_P8(v, 0), WL_P8(v, 8)::"memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -289,11 +304,21 @@ __device__ __forceinline__ long long quot(long long a, long long b) {  // a >= 0
   return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 
-// A run of key tiles [a, b) of one group: KV head kvh, query tiles qt0 .. qt0 + w - 1
+// A run of key tiles of one group: KV head kvh, query tiles qt0 .. qt0 + w - 1.
+// The TMA warp walks the CTA's share and hands the runs to the other warps
+// through shared memory, which keeps that state out of their registers.
 struct Run {
-  int i, kvh, qt0, w, a, b;
-  bool first, whole;  // the CTA's first run; the whole group
+  int nt;             // key tiles; 0: no further run
+  int key0;           // first key
+  int w;              // query tiles: 2, or 1
+  int len, keys;      // Req's
+  int row0, T;
+  int i, kvh, qt0;
+  int first, whole;   // the CTA's first run; the whole group
 };
+// Runs in flight: the TMA warp is ahead by no more than the ring's tiles, two
+// or more to a run, the others by one run.
+constexpr int kRuns = 10;
 
 // Walks the CTA's share [x, x1) of the laid-out key tiles; all threads alike.
 template <int HD, class Q>
@@ -316,13 +341,14 @@ struct Walk {
       r.w = min(S::NS, q.qt - r.qt0);
       const long long g0 = base + r.kvh * per + (long long)r.qt0 * q.kt;
       const long long g1 = g0 + (long long)r.w * q.kt, e = min(x1, g1);
-      r.i = i;
-      r.a = (int)((x - g0) >> (r.w - 1));  // w is 1 or 2
-      r.b = (int)((e - g0) >> (r.w - 1));
+      const int ta = (int)((x - g0) >> (r.w - 1)), tb = (int)((e - g0) >> (r.w - 1));  // w is 1 or 2
+      r.nt = tb - ta;
+      r.key0 = (q.tile0 + ta) * S::KT;
+      r.len = q.len, r.keys = q.keys, r.row0 = q.row0, r.T = q.T, r.i = i;
       r.first = x0 >= g0;
-      r.whole = r.a == 0 && r.b == q.kt;
+      r.whole = ta == 0 && tb == q.kt;
       x = e;
-      if (r.b > r.a) return true;
+      if (tb > ta) return true;
     }
     return false;
   }
@@ -358,6 +384,21 @@ __host__ inline Parts parts_at(void* ws, int ctas, int n, int hd, int prow) {
 
 __device__ __forceinline__ void st4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 
+template <int NSLOT>
+struct Small {  // behind the tiles in shared memory
+  uint64_t bars[2 * NSLOT + 20 + kRuns];
+  Run runs[kRuns];
+  union {
+    float half[2][2][128];  // [stream][half][row]
+    long long scan[kTaThreads / 32];  // at the start
+  };
+  long long base;
+  Req q;
+  int req, fail;
+  uint32_t tmem;
+};
+static_assert(kTaSmem + sizeof(Small<12>) <= 232448, "more than a CTA's shared memory");
+
 template <int HD, class Q>
 __global__ void __launch_bounds__(kTaThreads, 1)
     k_tree_attn(const TreeAttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -365,36 +406,37 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   using S = Shape<HD, Q>;
   using C = typename std::conditional<S::kSplit, __half, Q>::type;
   constexpr int KT = S::KT, NS = S::NS, NSLOT = S::kSlots, ATOMS = HD / 64, PAGES = KT / kKvPage;
-  extern __shared__ uint8_t ta_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t s_bars[2 * NSLOT + 10];
-  __shared__ uint32_t s_tmem;
-  __shared__ int s_fail;
-  __shared__ long long s_scan[kTaThreads / 32], s_base;
-  __shared__ int s_req;
-  __shared__ Req s_q;
-  __shared__ float2 s_ml[128];
-  const uint32_t full = sptr(s_bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
-                 pbar = sbar + 16, dbar = pbar + 16, obar = dbar + 8, endbar = obar + 8, xfull = endbar + 8, xempty = xfull + 8;
+  // everything lies in one dynamic block, which starts at the CTA's first byte
+  // of shared memory: 1024-byte aligned, as the swizzled tiles need it
+  extern __shared__ __align__(1024) uint8_t sm[];
+  Small<NSLOT>& sh = *reinterpret_cast<Small<NSLOT>*>(sm + kTaSmem);
+  if (sptr(sm) & 1023u) {
+    if (threadIdx.x == 0) parts.status[blockIdx.x] = 1;
+    return;
+  }
+  const uint32_t full = sptr(sh.bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
+                 pbar = sbar + 16, dbar = pbar + 16, obar = dbar + 8, endbar = obar + 8, xfull = endbar + 8, xempty = xfull + 16,
+                 hbar = xempty + 16, rbar = hbar + 64;
   const uint32_t qs = sptr(sm), ring = qs + S::kQBytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.heads / a.kv_heads;
 
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&s_tmem)) : "memory");
+  if (warp == kTaSoft + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (tid == 0) {
     for (int k = 0; k < NSLOT; k++) bar_init(full + 8 * k, 1), bar_init(empty + 8 * k, 1);
-    bar_init(qbar, 256);
-    for (int k = 0; k < 2; k++) bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 128);
+    bar_init(qbar, kTaSoft);
+    for (int k = 0; k < 2; k++)
+      bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 8), bar_init(xfull + 8 * k, 4), bar_init(xempty + 8 * k, 4);
+    for (int k = 0; k < 8; k++) bar_init(hbar + 8 * k, 2);
+    for (int k = 0; k < kRuns; k++) bar_init(rbar + 8 * k, 1);
     bar_init(dbar, 1);
     bar_init(obar, 1);
     bar_init(endbar, 1);
-    bar_init(xfull, 128);
-    bar_init(xempty, 128);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    s_fail = 0;
+    sh.fail = 0;
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mk) : "memory");
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mv) : "memory");
   }
@@ -402,7 +444,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   pdl_trigger();
 
   // this CTA's share of the key tiles: the total, then the request it starts in
-  Walk<HD, Q> walk;
+  long long share0, share1;
   {
     auto block_sum = [&](long long v, long long& before) {  // the sum, and that of the threads before this one
       long long x = v;
@@ -412,12 +454,12 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (lane >= o) x += y;
       }
       __syncthreads();
-      if (lane == 31) s_scan[warp] = x;
+      if (lane == 31) sh.scan[warp] = x;
       __syncthreads();
       long long w = 0, all = 0;
       for (int k = 0; k < kTaThreads / 32; k++) {
         if (k == warp) w = all;
-        all += s_scan[k];
+        all += sh.scan[k];
       }
       before = w + x - v;
       return all;
@@ -430,8 +472,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       total += block_sum(u, before);
     }
     const long long per = total > 0 ? quot(total + gridDim.x - 1, gridDim.x) : 1;
-    walk.x0 = walk.x = min(total, per * blockIdx.x);
-    walk.x1 = min(total, walk.x0 + per);
+    share0 = min(total, per * blockIdx.x);
+    share1 = min(total, share0 + per);
     long long sum = 0;
     for (int i0 = 0; i0 < a.n; i0 += kTaThreads) {
       const int i = i0 + tid;
@@ -442,7 +484,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         all = block_sum(u, before);
       }
       before += sum;
-      if (walk.x >= before && walk.x < before + u) s_req = i, s_base = before, s_q = q;
+      if (share0 >= before && share0 < before + u) sh.req = i, sh.base = before, sh.q = q;
       if (blockIdx.x == 0 && i < a.n) parts.start[i] = before;
       sum += all;
     }
@@ -451,34 +493,46 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = s_tmem;
-  if (walk.x < walk.x1) {
-    walk.i = s_req;
-    walk.base = s_base;
-    walk.q = s_q;
-  }
-  Run run;
+  const uint32_t tmem = sh.tmem;
+  // run r of the CTA, once the TMA warp has put it down; null when a wait gave up
+  auto get_run = [&](uint32_t r) -> const Run* {
+    const uint32_t k = r % kRuns;
+    return bar_wait(rbar + 8 * k, (r / kRuns) & 1, &sh.fail) ? &sh.runs[k] : nullptr;
+  };
 
-  if (warp == 8) {
+  if (warp == kTaSoft) {
     // ------------------------------------------------------------ TMA
     // tiles in the order the products use them: a pair of query tiles K0 V0 K1
     // V1 ..., a single one K0 K1 V0 K2 V1 ...
-    uint32_t seq = 0;
+    uint32_t seq = 0, nr = 0;
+    Walk<HD, Q> walk;
+    walk.x0 = walk.x = share0;
+    walk.x1 = share1;
+    if (share0 < share1) walk.i = sh.req, walk.base = sh.base, walk.q = sh.q;
+    Run run;
+    auto hand_over = [&]() {
+      if (lane == 0) {
+        sh.runs[nr % kRuns] = run;
+        bar_arrive(rbar + 8 * (nr % kRuns));
+      }
+      nr++;
+    };
     const int rows_end = a.n_pages * a.kv_heads * kKvPage;  // past the cache: read as zeros
     bool ok = true;
     while (ok && walk.next(a, run)) {
-      const int nt = run.b - run.a;
+      hand_over();
+      const int nt = run.nt;
       const int* table = a.tables + (size_t)run.i * a.ld_tables;
       auto load = [&](const CUtensorMap* map, int tile) {
         if (!ok) return;
-        const int pg = (walk.q.tile0 + run.a + tile) * PAGES + lane;
+        const int pg = run.key0 / kKvPage + tile * PAGES + lane;
         int row = rows_end;
-        if (lane < PAGES && pg < a.max_pages && pg * kKvPage < walk.q.keys) {
+        if (lane < PAGES && pg < a.max_pages && pg * kKvPage < run.keys) {
           const int id = table[pg];
           if (id >= 0 && id < a.n_pages) row = (id * a.kv_heads + run.kvh) * kKvPage;
         }
         const uint32_t slot = seq % NSLOT, bar = full + 8 * slot;
-        if (seq >= NSLOT) ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * slot, (seq / NSLOT - 1) & 1, &s_fail));
+        if (seq >= NSLOT) ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * slot, (seq / NSLOT - 1) & 1, &sh.fail));
         if (!ok) return;
         if (lane == 0)
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)S::kSlot)
@@ -507,100 +561,138 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
       }
     }
+    run.nt = 0;
+    hand_over();
     // every copy has landed before the CTA ends
     for (uint32_t k = seq > NSLOT ? seq - NSLOT : 0; k < seq; k++) {
       int dummy = 0;
       bar_wait(full + 8 * (k % NSLOT), (k / NSLOT) & 1, &dummy);
     }
-  } else if (warp == 9) {
+  } else if (warp == kTaSoft + 1) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
-      uint32_t seq = 0;          // tiles of the ring used up by earlier runs
-      uint32_t np[2] = {0, 0};   // P tiles taken from each buffer
-      uint32_t runs = 0;
-      bool ok = true;
-      while (ok && walk.next(a, run)) {
-        const int nt = run.b - run.a, pair = run.w == 2, nu = pair ? 2 * nt : nt;
-        // place in the ring's order of the K and V tile of unit u
-        auto k_at = [&](int u) { return pair ? (uint32_t)(u >> 1) * 2 : u < 2 ? (uint32_t)u : (uint32_t)(2 * u - 1); };
-        auto v_at = [&](int u) {
-          return pair ? (uint32_t)(u >> 1) * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt);
-        };
-        auto scores = [&](int u) {  // S[u % 2] = Q K^T
-          const uint32_t k = seq + k_at(u), slot = k % NSLOT;
-          if (!(ok = ok && bar_wait(full + 8 * slot, (k / NSLOT) & 1, &s_fail))) return;
-          fence_after();
-          const uint32_t kb = ring + slot * S::kSlot, qb = qs + (pair ? (u & 1) * S::kQTile : 0);
-          const uint32_t d = tmem + (u & 1) * KT;
+    // The whole warp follows the schedule, so that operands are formed in
+    // uniform registers; one elected lane issues.  (With the loop run by a
+    // single lane a product took about 90 cycles to issue.)
+    const bool lead = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    uint32_t seq = 0;          // tiles of the ring used up by earlier runs
+    uint32_t np[2] = {0, 0};   // P tiles taken from each buffer
+    uint32_t runs = 0;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      return ok = ok && __all_sync(0xffffffffu, bar_wait(bar, parity, &sh.fail));
+    };
+    while (true) {
+      const Run* run = get_run(runs);
+      ok = __all_sync(0xffffffffu, run != nullptr);
+      if (!ok) break;
+      const int nt = __shfl_sync(0xffffffffu, run->nt, 0);
+      const bool pair = __shfl_sync(0xffffffffu, run->w, 0) == 2;
+      if (nt == 0) break;
+      const int nu = pair ? 2 * nt : nt;
+      // place in the ring's order of the K and V tile of unit u
+      auto k_at = [&](int u) { return pair ? (uint32_t)(u >> 1) * 2 : u < 2 ? (uint32_t)u : (uint32_t)(2 * u - 1); };
+      auto v_at = [&](int u) {
+        return pair ? (uint32_t)(u >> 1) * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt);
+      };
+      auto scores = [&](int u) {  // S[u % 2] = Q K^T
+        const uint32_t k = seq + k_at(u), slot = k % NSLOT;
+        if (!wait(full + 8 * slot, (k / NSLOT) & 1)) return;
+        fence_after();
+        const uint32_t kb = desc_lo(ring + slot * S::kSlot, 16);
+        const uint32_t qb = desc_lo(qs + (pair ? (u & 1) * S::kQTile : 0), 16), d = tm + (u & 1) * KT;
+        if (lead) {
 #pragma unroll
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
 #pragma unroll
-            for (int ks = 0; ks < HD / 16; ks++) {
-              const uint32_t o = (ks >> 2) * 128 * 128 + (ks & 3) * 32, ok_ = (ks >> 2) * KT * 128 + (ks & 3) * 32;
-              mma_ss(d, sw128_desc(qb + (S::kSplit && !w ? NS * S::kQTile : 0) + o, 16, 1024),
-                     sw128_desc(kb + ok_, 16, 1024), S::kIdescS,
-                     w || ks ? 1u : 0u);
-            }
+            for (int ks = 0; ks < HD / 16; ks++)
+              // the low words first: sums are cut off rather than rounded, and
+              // that costs least while they are small
+              mma_ss(d, qb + (((S::kSplit && !w ? NS * S::kQTile : 0) + (ks >> 2) * 128 * 128 + (ks & 3) * 32) >> 4),
+                     kb + (((ks >> 2) * KT * 128 + (ks & 3) * 32) >> 4), S::kIdescS, w || ks ? 1u : 0u);
           mma_commit(sbar + 8 * (u & 1));
           if (!pair || (u & 1)) mma_commit(empty + 8 * slot);
-        };
-        if (!(ok = bar_wait(qbar, runs & 1, &s_fail))) break;
-        runs++;
+        }
+      };
+      if (!wait(qbar, runs & 1)) break;
+      runs++;
+      fence_after();
+      scores(0);
+      if (nu > 1) scores(1);
+      for (int u = 0; ok && u < nu; u++) {
+        const int b = u & 1;
+        const uint32_t k = seq + v_at(u), slot = k % NSLOT;
+        if (!wait(pbar + 8 * b, np[b]++ & 1) || !wait(full + 8 * slot, (k / NSLOT) & 1)) break;
         fence_after();
-        scores(0);
-        if (nu > 1) scores(1);
-        for (int u = 0; ok && u < nu; u++) {
-          const int b = u & 1;
-          const uint32_t k = seq + v_at(u), slot = k % NSLOT;
-          ok = bar_wait(pbar + 8 * b, np[b]++ & 1, &s_fail) && bar_wait(full + 8 * slot, (k / NSLOT) & 1, &s_fail);
-          if (!ok) break;
-          fence_after();
-          const uint32_t vb = ring + slot * S::kSlot, d = tmem + S::kO + (NS == 2 ? b * HD : 0), p = tmem + b * KT;
-          const bool fresh = NS == 2 ? u < 2 : u == 0;
+        const uint32_t vb = desc_lo(ring + slot * S::kSlot, KT * 128);
+        const uint32_t d = tm + S::kO + (NS == 2 ? b * HD : 0), p = tm + b * KT;
+        const uint32_t acc = (NS == 2 ? u < 2 : u == 0) ? 0u : 1u;
+        if (lead) {
 #pragma unroll
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
 #pragma unroll
             for (int ks = 0; ks < KT / 16; ks++)
-              // the low words first: sums are cut off rather than rounded, and
-              // that costs least while they are small
-              mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8 + (S::kSplit && !w ? 16 : 0),
-                     sw128_desc(vb + ks * 16 * 128, KT * 128, 1024), S::kIdescO, fresh && !w && !ks ? 0u : 1u);
+              mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8 + (S::kSplit && !w ? 16 : 0), vb + (ks * 16 * 128 >> 4),
+                     S::kIdescO, w || ks ? 1u : acc);
           if (!pair || b) mma_commit(empty + 8 * slot);
           if (NS == 1) mma_commit(obar);
-          if (u + 2 < nu) scores(u + 2);
         }
-        if (ok) mma_commit(dbar);
-        seq += 2 * nt;
+        if (u + 2 < nu) scores(u + 2);
       }
-      if (!ok) {  // products in flight finish before TMEM is given back
-        mma_commit(endbar);
-        int dummy = 0;
-        bar_wait(endbar, 0, &dummy);
-      }
+      if (!ok) break;
+      if (lead) mma_commit(dbar);
+      seq += 2 * nt;
+    }
+    if (!ok && lead) {  // products in flight finish before TMEM is given back
+      mma_commit(endbar);
+      int dummy = 0;
+      bar_wait(endbar, 0, &dummy);
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
-    const int t = warp >> 2, wt = tid & 127;                 // stream; row of its query tile
+    // stream t; half hf of the key tile's columns (and of O's); row wt of the query tile
+    const int t = warp >> 3, hf = (warp >> 2) & 1, wt = (warp & 3) * 32 + lane;
+    constexpr int CW = KT / 2, OW = HD / 2;  // columns of S and of O that a thread takes
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t oth = hbar + 8 * (t * 4 + (warp & 3));  // meets the other half's warp
+    const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0) + hf * OW;
     const float c = a.scale * 1.4426950408889634f;
     uint32_t ns[2] = {0, 0}, runs = 0, no = 0, seq = 0;
     uint32_t nx = 0;           // exchanges between the streams
+    uint32_t nh = 0;           // and between the halves
     bool ok = true;
     auto wait_warp = [&](uint32_t bar, uint32_t parity) {  // the same answer for the whole warp
-      return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, &s_fail));
+      return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, &sh.fail));
     };
-    while (ok && walk.next(a, run)) {
-      const Req& rq = walk.q;
-      const int nt = run.b - run.a, pair = run.w == 2, nu = pair ? 2 * nt : nt;
-      // queries: thread e of 256 copies 16-byte pieces of the (row, head) pairs
+    auto arrive_warp = [&](uint32_t bar) {
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar);
+    };
+    auto meet = [&]() {
+      arrive_warp(oth);
+      ok = wait_warp(oth, nh++ & 1);
+    };
+    // this row's value of the other half.  The next call writes over it: between
+    // two calls lie a product or a meet(), for which the other half has read.
+    auto swap_half = [&](float v) {
+      sh.half[t][hf][wt] = v;
+      meet();
+      return sh.half[t][hf ^ 1][wt];
+    };
+    while (true) {
+      const Run* rp = get_run(runs);
+      if (!__all_sync(0xffffffffu, rp != nullptr) || rp->nt == 0) break;
+      const Run& run = *rp;
+      const int nt = run.nt, pair = run.w == 2, nu = pair ? 2 * nt : nt, len = run.len, first = run.key0;
+      // queries: the threads copy 16-byte pieces of the (row, head) pairs
       {
-        const int m0 = run.qt0 * 128, mn = min(run.w * 128, rq.T * group - m0);
+        const int m0 = run.qt0 * 128, mn = min(run.w * 128, run.T * group - m0);
         const Q* src = (const Q*)a.q + (size_t)run.kvh * group * HD;
-        for (int e = tid; e < mn * (HD / 8); e += 256) {
+        for (int e = tid; e < mn * (HD / 8); e += kTaSoft * 32) {
           const int m = e / (HD / 8), ch = e - m * (HD / 8);
           const int j = (m0 + m) / group, g = (m0 + m) - j * group;
-          const Q* p = src + (size_t)(rq.row0 + j) * a.ldq + (size_t)g * HD + ch * 8;
+          const Q* p = src + (size_t)(run.row0 + j) * a.ldq + (size_t)g * HD + ch * 8;
           const int row = m & 127;
           uint8_t* d = sm + (m >> 7) * S::kQTile + (ch >> 3) * 128 * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
           if constexpr (S::kSplit) {
@@ -623,21 +715,21 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       }
       fence_async();
       fence_before();
-      bar_arrive(qbar);
+      arrive_warp(qbar);
 
       const int m = (run.qt0 + (pair ? t : 0)) * 128 + wt;
       const int j = m / group, g = m - j * group;
-      const bool live = m < rq.T * group;
-      const int row = rq.row0 + (live ? j : 0);
+      const bool live = m < run.T * group;
+      const int row = run.row0 + (live ? j : 0);
       int pos = live ? a.pos[row] : -1;
-      if (pos >= 0 && pos < rq.len) pos = rq.len;
+      if (pos >= 0 && pos < len) pos = len;
       const bool warp_live = __any_sync(0xffffffffu, live);
       // a page outside the cache: then every tile looks at its pages
       const int* table = a.tables + (size_t)run.i * a.ld_tables;
       bool holes = false;
       {
-        const int p1 = min((rq.tile0 + run.b) * PAGES, (rq.keys + kKvPage - 1) / kKvPage);
-        for (int p = (rq.tile0 + run.a) * PAGES + lane; p < p1; p += 32) {
+        const int p1 = min((first + nt * KT) / kKvPage, (run.keys + kKvPage - 1) / kKvPage);
+        for (int p = first / kKvPage + lane; p < p1; p += 32) {
           const int id = table[p];
           holes |= id < 0 || id >= a.n_pages;
         }
@@ -648,10 +740,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         uint32_t see = 0;
         if (pos < 0) return see;
         // cached tokens: a range
-        const int lo = a.window > 0 ? max(pos - a.window + 1 - k0, 0) : 0, hi = min(rq.len - k0, 32);
+        const int lo = a.window > 0 ? max(pos - a.window + 1 - k0, 0) : 0, hi = min(len - k0, 32);
         if (hi > lo) see = (hi >= 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
         // the step's own: bits of the mask (c0: node of the word's first key)
-        const int c0 = k0 - rq.len, cn = rq.keys - rq.len;
+        const int c0 = k0 - len, cn = run.keys - len;
         if (c0 > -32 && c0 < cn) {
           uint32_t own;
           if (!a.mask) {
@@ -665,14 +757,14 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           if (a.window > 0)
             for (uint32_t left = own; left; left &= left - 1) {
               const int bit = __ffs(left) - 1;
-              if (a.pos[rq.row0 + c0 + bit] <= pos - a.window) own &= ~(1u << bit);
+              if (a.pos[run.row0 + c0 + bit] <= pos - a.window) own &= ~(1u << bit);
             }
           see |= own;
         }
         if (holes) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            const int pg = k0 / kKvPage + h, id = pg * kKvPage < rq.keys ? table[pg] : -1;
+            const int pg = k0 / kKvPage + h, id = pg * kKvPage < run.keys ? table[pg] : -1;
             if (id < 0 || id >= a.n_pages) see &= ~(0xffffu << (16 * h));
           }
         }
@@ -681,111 +773,114 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       float mx = -INFINITY, l = 0.f;
       const int step = NS == 2 ? 2 : 1;
       for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step) {
-        const int b = u & 1, tile = pair ? u >> 1 : u, key0 = (rq.tile0 + run.a + tile) * KT;
+        const int b = u & 1, tile = pair ? u >> 1 : u, key0 = first + tile * KT;
         ok = wait_warp(sbar + 8 * b, ns[b]++ & 1);
         if (!ok) break;
         fence_after();
-        const uint32_t sp = tmem + lanes + b * KT;
+        const uint32_t sp = tmem + lanes + b * KT + hf * CW;
         if (warp_live) {
           // which keys the row sees, when it is not all of them
-          const bool plain = key0 + KT <= rq.len && !holes && (a.window <= 0 || key0 > pos - a.window) && pos >= 0;
+          const bool plain = key0 + KT <= len && !holes && (a.window <= 0 || key0 > pos - a.window) && pos >= 0;
           const bool masked = !__all_sync(0xffffffffu, plain || !live);
-          uint32_t see[KT / 32];
+          uint32_t see[CW / 32];
           if (masked) {
 #pragma unroll
-            for (int k = 0; k < KT / 32; k++) see[k] = visible(key0 + 32 * k);
+            for (int k = 0; k < CW / 32; k++) see[k] = visible(key0 + hf * CW + 32 * k);
             __syncwarp();
           }
-          // S comes in 32 columns at a time, once for the maximum and once for P
-          float s[32], top = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < KT / 32; k++) {
+          // the scores come in 32 at a time, for the maximum and again for P:
+          // held in between, they would push the loop's state out of registers
+          float s[32], top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto load = [&](int k) {
             tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
             tm_wait_ld(reinterpret_cast<uint32_t*>(s));
             if (masked) {
 #pragma unroll
               for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
             }
-            float t4[4] = {s[0], s[1], s[2], s[3]};
+          };
 #pragma unroll
-            for (int e = 4; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], s[e]);
-            top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+          for (int k = 0; k < CW / 32; k++) {
+            load(k);
+#pragma unroll
+            for (int e = 0; e < 32; e++) top4[e & 3] = fmaxf(top4[e & 3], s[e]);
           }
-          top *= c;
+          float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+          // with one stream the scores do not say that the last product is done
+          if (NS == 1 && u > 0 && !(ok = wait_warp(obar, no++ & 1))) break;
+          top = fmaxf(top, swap_half(top)) * c;
+          if (!ok) break;
           // follow the maximum; O and l are rescaled only past the lag
           float scale = 1.f;
-          if (l == 0.f) {
-            mx = fmaxf(mx, top);
+          if (mx == -INFINITY) {
+            mx = top;
           } else if (live && top > mx + kTaLag) {
             scale = ex2(mx - top);
             mx = top;
             l *= scale;
           }
-          if (NS == 1 && u > 0 && !(ok = wait_warp(obar, no++ & 1))) break;
           if (__any_sync(0xffffffffu, scale != 1.f)) {
             fence_after();
-            const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0);
 #pragma unroll 1
-            for (int k = 0; k < HD / 32; k++) {
-              tm_ld32(op + k * 32, reinterpret_cast<uint32_t*>(s));
-              tm_wait_ld(reinterpret_cast<uint32_t*>(s));
+            for (int k = 0; k < OW / 16; k++) {
+              uint32_t v[16];
+              tm_ld16(op + k * 16, v);
+              tm_wait_ld16(v);
 #pragma unroll
-              for (int e = 0; e < 32; e++) s[e] *= scale;
-              tm_st32(op + k * 32, reinterpret_cast<uint32_t*>(s));
+              for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
+              tm_st16(op + k * 16, v);
             }
           }
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < KT / 32; k++) {
-            tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
-            tm_wait_ld(reinterpret_cast<uint32_t*>(s));
-            if (masked) {
+          for (int k = 0; k < CW / 32; k++) {
+            if (CW > 32) load(k);
+            // over the scores they came from: 16 columns of high words, then low ones
 #pragma unroll
-              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
-            }
-            uint32_t hi[16], lo[16];
+            for (int h = 0; h < 2; h++) {
+              uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-              const float p0 = ex2(fmaf(s[2 * e], c, off)), p1 = ex2(fmaf(s[2 * e + 1], c, off));
-              sum[(2 * e) & 3] += p0;
-              sum[(2 * e + 1) & 3] += p1;
-              hi[e] = pack2(p0, p1, C());
-              if constexpr (S::kSplit) {
-                __half2 h;
-                memcpy(&h, &hi[e], 4);
-                const float2 f = __half22float2(h);
-                lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
+              for (int e = 0; e < 8; e++) {
+                const float p0 = ex2(fmaf(s[16 * h + 2 * e], c, off)), p1 = ex2(fmaf(s[16 * h + 2 * e + 1], c, off));
+                sum[(2 * e) & 3] += p0;
+                sum[(2 * e + 1) & 3] += p1;
+                hi[e] = pack2(p0, p1, C());
+                if constexpr (S::kSplit) {
+                  __half2 x;
+                  memcpy(&x, &hi[e], 4);
+                  const float2 f = __half22float2(x);
+                  lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
+                }
               }
+              tm_st8(sp + k * 32 + h * 8, hi);
+              if constexpr (S::kSplit) tm_st8(sp + k * 32 + 16 + h * 8, lo);
             }
-            // over the scores they came from: the high words, then the low ones
-            tm_st16(sp + k * 32, hi);
-            if constexpr (S::kSplit) tm_st16(sp + k * 32 + 16, lo);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tm_wait_st();
         } else if (NS == 1 && u > 0) {
           no++;
         }
-        if (key0 + KT > rq.len) {
+        if (hf == 0 && key0 + KT > len) {
           // V rows that no row sees: keys past the end, nodes in nobody's mask.
           // A warp takes 32 keys, its lanes the request's rows.
           const int k0 = key0 + (wt & ~31);
           bool dead = false;
           if (wt < KT) {
             uint32_t seen = 0;
-            if (!a.mask || k0 + 32 <= rq.len) {
+            if (!a.mask || k0 + 32 <= len) {
               seen = 0xffffffffu;
-            } else if (k0 < rq.keys) {
+            } else if (k0 < run.keys) {
 #pragma unroll 2
-              for (int r = lane; r < rq.T; r += 32) {
-                const uint32_t bits = mask_bits(a, rq.row0 + r, k0 - rq.len);
-                if (a.pos[rq.row0 + r] >= 0) seen |= bits;
+              for (int r = lane; r < run.T; r += 32) {
+                const uint32_t bits = mask_bits(a, run.row0 + r, k0 - len);
+                if (a.pos[run.row0 + r] >= 0) seen |= bits;
               }
               seen = __reduce_or_sync(0xffffffffu, seen);
-              if (k0 < rq.len) seen |= (1u << (rq.len - k0)) - 1u;  // cached tokens of the word
+              if (k0 < len) seen |= (1u << (len - k0)) - 1u;  // cached tokens of the word
             }
-            dead = key0 + wt >= rq.keys || !(seen >> lane & 1u);
+            dead = key0 + wt >= run.keys || !(seen >> lane & 1u);
           }
           const uint32_t k = seq + (pair ? (uint32_t)tile * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt));
           const uint32_t slot = k % NSLOT;
@@ -802,7 +897,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           fence_async();
         }
         fence_before();
-        bar_arrive(pbar + 8 * b);
+        arrive_warp(pbar + 8 * b);
       }
       seq += 2 * nt;
       if (!ok) break;
@@ -810,84 +905,88 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (!ok) break;
       if (NS == 1) no++;  // the last product's phase
       fence_after();
-      const bool worked = NS == 2 ? t < nu : t == 0;
+      if (!(NS == 2 ? t < nu : t == 0)) continue;  // no tile for this stream
+      l += swap_half(l);
+      if (!ok) break;
       const bool merge = NS == 2 && run.whole && !pair && nu > 1;  // two streams of one row, joined here
-      const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0);
-      float* xb = reinterpret_cast<float*>(sm + S::kQTile);  // [32][128]: the second query tile's place is free
+      float* xb = reinterpret_cast<float*>(sm + S::kQTile) + hf * 16 * 128;  // the second query tile's place is free
       float own = 1.f, other = 0.f;
-      if (merge && t == 1) {
-        s_ml[wt] = make_float2(mx, l);
+      if (merge && t == 1) {  // (m, l) for the other stream
+        meet();
+        sh.half[1][hf][wt] = hf ? l : mx;
+        if (ok) meet();
+        if (!ok) break;
       }
       float* po = nullptr;
-      if (worked && !run.whole && live && wt < parts.prow) {
+      if (!run.whole && live && wt < parts.prow) {
         const size_t at = (((size_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * 2 + t) * parts.prow + wt;
-        po = parts.o + at * HD;
-        *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(mx, l);
+        po = parts.o + at * HD + hf * OW;
+        if (hf == 0) *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(mx, l);
       }
-      Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD;
+      Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD + hf * OW;
       const bool write = run.whole && live && !(merge && t == 1);
 #pragma unroll 1
-      for (int k = 0; worked && k < HD / 32; k++) {
-        float v[32];
+      for (int k = 0; k < OW / 16; k++) {
+        float v[16];
         __syncwarp();
         if (warp_live) {
-          tm_ld32(op + k * 32, reinterpret_cast<uint32_t*>(v));
-          tm_wait_ld(reinterpret_cast<uint32_t*>(v));
+          tm_ld16(op + k * 16, reinterpret_cast<uint32_t*>(v));
+          tm_wait_ld16(reinterpret_cast<uint32_t*>(v));
         }
         if (merge) {
           if (t == 1) {
-            if (nx > 0 && !(ok = wait_warp(xempty, (nx - 1) & 1))) break;
+            if (nx > 0 && !(ok = wait_warp(xempty + 8 * hf, (nx - 1) & 1))) break;
 #pragma unroll
-            for (int e = 0; e < 32; e++) xb[e * 128 + wt] = v[e];
-            bar_arrive(xfull);
+            for (int e = 0; e < 16; e++) xb[e * 128 + wt] = v[e];
+            arrive_warp(xfull + 8 * hf);
           } else {
-            if (!(ok = wait_warp(xfull, nx & 1))) break;
+            if (!(ok = wait_warp(xfull + 8 * hf, nx & 1))) break;
             if (k == 0) {
-              const float2 ml = s_ml[wt];
+              const float2 ml = make_float2(sh.half[1][0][wt], sh.half[1][1][wt]);
               const float mn = fmaxf(mx, ml.x);
               own = l == 0.f ? 0.f : ex2(mx - mn);
               other = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
               l = l * own + ml.y * other;
             }
 #pragma unroll
-            for (int e = 0; e < 32; e++) v[e] = v[e] * own + xb[e * 128 + wt] * other;
-            bar_arrive(xempty);
+            for (int e = 0; e < 16; e++) v[e] = v[e] * own + xb[e * 128 + wt] * other;
+            arrive_warp(xempty + 8 * hf);
           }
           nx++;
         }
         if (po) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) st4(po + k * 32 + e, v + e);
+          for (int e = 0; e < 16; e += 4) st4(po + k * 16 + e, v + e);
         }
         if (write) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
           if (l == 0.f) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) v[e] = 0.f;
+            for (int e = 0; e < 16; e++) v[e] = 0.f;
           }
           if constexpr (S::kSplit) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) v[e] *= inv;
+            for (int e = 0; e < 16; e++) v[e] *= inv;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) st4((float*)out + k * 32 + e, v + e);
+            for (int e = 0; e < 16; e += 4) st4((float*)out + k * 16 + e, v + e);
           } else {
-            uint32_t w[16];
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) w[e] = pack2(v[2 * e] * inv, v[2 * e + 1] * inv, C());
+            for (int e = 0; e < 8; e++) w[e] = pack2(v[2 * e] * inv, v[2 * e + 1] * inv, C());
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<uint4*>(out + k * 32 + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+            for (int e = 0; e < 8; e += 4)
+              *reinterpret_cast<uint4*>(out + k * 16 + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
           }
         }
       }
       // the exchange's last round has been read before its place is written again
-      if (merge && t == 1 && ok) ok = wait_warp(xempty, (nx - 1) & 1);
+      if (merge && t == 1 && ok) ok = wait_warp(xempty + 8 * hf, (nx - 1) & 1);
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
-  if (tid == 0) parts.status[blockIdx.x] = s_fail;
+  if (warp == kTaSoft + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+  if (tid == 0) parts.status[blockIdx.x] = sh.fail;
 }
 
 // Merges the parts of the groups that were cut: a warp per (row, head), its
@@ -1005,7 +1104,7 @@ int launch_t(const TreeAttnArgs& a, cudaStream_t st) {
   WL_TRY(cache_map(&mv, a.cache_v, S::kBf16, HD, rows));
   const int ctas = device_sms();
   const Parts parts = parts_at(a.workspace, ctas, a.n, HD, part_rows(a.rows, a.heads / a.kv_heads));
-  constexpr int smem = kTaSmem + 1024;
+  constexpr int smem = kTaSmem + (int)sizeof(Small<S::kSlots>);
   if (first_use_on_device((const void*)k_tree_attn<HD, Q>))
     WL_CUDA_TRY(cudaFuncSetAttribute(k_tree_attn<HD, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   WL_TRY(launch_k(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
