@@ -22,10 +22,11 @@
 //   others     softmax, two threads per query row (half of a key tile's columns
 //              each): S from TMEM into registers, mask, running maximum and sum,
 //              P back over S.
-// They work on two streams, so that one's softmax runs under the other's
-// products: the two query tiles of a pair over the same keys or, for a single
-// query tile, even and odd key tiles, merged with the parts.  head_dim 256 has
-// room in TMEM for one O only: one stream, with S double-buffered.
+// They work on two streams, each with two S buffers, so that the scores run
+// ahead of the softmax and one stream's softmax under the other's products: the
+// two query tiles of a pair over the same keys or, for a single query tile,
+// even and odd key tiles, merged at the end.  head_dim 256 has room in TMEM for
+// one O only: one stream.
 // The maximum that P is taken against follows the true one with a lag of up to
 // 2^6 (O is rescaled only past that), and P is scaled by 2^8 where it is f16, so
 // that it stays clear of both ends of the type; both factors cancel in o / l.
@@ -134,20 +135,24 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
 
 // ---------------------------------------------------------------- tcgen05
 constexpr int kTaSoft = 16;          // softmax warps: 2 streams x 2 halves of the key tile x 4 lane quarters
-constexpr int kTaThreads = (kTaSoft + 2) * 32;
-constexpr int kTaSmem = 224 * 1024;   // query tiles, then the ring of K / V tiles
+constexpr int kTaLoad = 2;           // TMA warps, each with half of a tile's pages
+constexpr int kTaThreads = (kTaSoft + kTaLoad + 1) * 32;
+constexpr int kTaSmem = 232448;      // a CTA's shared memory: query tiles, the ring of K / V tiles, Small
 constexpr int kTaLag = 6;             // log2 of the lag of the maximum
 
 template <int HD, class Q>
 struct Shape {
   static constexpr bool kSplit = sizeof(Q) == 4;       // f32 queries as two f16 words
-  static constexpr int KT = HD == 256 ? 64 : 128;      // keys per tile
+  static constexpr int KT = 64;                        // keys per tile
   static constexpr int NS = HD == 256 ? 1 : 2;         // streams
+  static constexpr int NB = 2 * NS;                    // S buffers, two per stream
   static constexpr int kQTile = 128 * HD * 2;          // bytes of a query tile (one word)
   static constexpr int kQBytes = kQTile * NS * (kSplit ? 2 : 1);
   static constexpr int kSlot = KT * HD * 2;            // bytes of a K or V tile
-  static constexpr int kSlots = (kTaSmem - kQBytes) / kSlot;
-  static constexpr int kO = 256;                       // TMEM column of O; S at 0 and KT
+  static constexpr int kFit = (kTaSmem - kQBytes - (NS == 2 ? 5376 : 3072)) / kSlot;
+  static constexpr int kSlots = kFit < 12 ? kFit : 12;
+  static constexpr int kTiles = kQBytes + kSlots * kSlot;
+  static constexpr int kO = 256;                       // TMEM column of O; S buffers from 0
   static constexpr bool kBf16 = std::is_same<Q, __nv_bfloat16>::value;
   static constexpr float kShift = kBf16 ? 0.f : 8.f;   // log2 of P's scale
   static constexpr uint32_t kType = kBf16 ? (1u << 7) | (1u << 10) : 0u;
@@ -384,12 +389,13 @@ __host__ inline Parts parts_at(void* ws, int ctas, int n, int hd, int prow) {
 
 __device__ __forceinline__ void st4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 
-template <int NSLOT>
+template <int HD, class Q>
 struct Small {  // behind the tiles in shared memory
-  uint64_t bars[2 * NSLOT + 20 + kRuns];
+  static constexpr int NSLOT = Shape<HD, Q>::kSlots, NS = Shape<HD, Q>::NS;
+  uint64_t bars[2 * NSLOT + 26 + kRuns];
   Run runs[kRuns];
   union {
-    float half[2][2][128];  // [stream][half][row]
+    float half[2][NS][2][128];  // [parity of the exchange][stream][half][row]
     long long scan[kTaThreads / 32];  // at the start
   };
   long long base;
@@ -397,7 +403,6 @@ struct Small {  // behind the tiles in shared memory
   int req, fail;
   uint32_t tmem;
 };
-static_assert(kTaSmem + sizeof(Small<12>) <= 232448, "more than a CTA's shared memory");
 
 template <int HD, class Q>
 __global__ void __launch_bounds__(kTaThreads, 1)
@@ -405,35 +410,35 @@ __global__ void __launch_bounds__(kTaThreads, 1)
                 const Parts parts) {
   using S = Shape<HD, Q>;
   using C = typename std::conditional<S::kSplit, __half, Q>::type;
-  constexpr int KT = S::KT, NS = S::NS, NSLOT = S::kSlots, ATOMS = HD / 64, PAGES = KT / kKvPage;
+  constexpr int KT = S::KT, NS = S::NS, NB = S::NB, NSLOT = S::kSlots, ATOMS = HD / 64, PAGES = KT / kKvPage;
   // everything lies in one dynamic block, which starts at the CTA's first byte
   // of shared memory: 1024-byte aligned, as the swizzled tiles need it
   extern __shared__ __align__(1024) uint8_t sm[];
-  Small<NSLOT>& sh = *reinterpret_cast<Small<NSLOT>*>(sm + kTaSmem);
+  Small<HD, Q>& sh = *reinterpret_cast<Small<HD, Q>*>(sm + S::kTiles);
+  static_assert(S::kTiles + sizeof(Small<HD, Q>) <= kTaSmem, "more than a CTA's shared memory");
   if (sptr(sm) & 1023u) {
     if (threadIdx.x == 0) parts.status[blockIdx.x] = 1;
     return;
   }
   const uint32_t full = sptr(sh.bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
-                 pbar = sbar + 16, dbar = pbar + 16, obar = dbar + 8, endbar = obar + 8, xfull = endbar + 8, xempty = xfull + 16,
-                 hbar = xempty + 16, rbar = hbar + 64;
+                 pbar = sbar + 32, dbar = pbar + 32, obar = dbar + 8, endbar = obar + 16, xfull = endbar + 8,
+                 xempty = xfull + 16, hbar = xempty + 16, rbar = hbar + 64;
   const uint32_t qs = sptr(sm), ring = qs + S::kQBytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.heads / a.kv_heads;
 
-  if (warp == kTaSoft + 1) {
+  if (warp == kTaSoft + kTaLoad) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (tid == 0) {
-    for (int k = 0; k < NSLOT; k++) bar_init(full + 8 * k, 1), bar_init(empty + 8 * k, 1);
+    for (int k = 0; k < NSLOT; k++) bar_init(full + 8 * k, kTaLoad), bar_init(empty + 8 * k, 1);
     bar_init(qbar, kTaSoft);
-    for (int k = 0; k < 2; k++)
-      bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 8), bar_init(xfull + 8 * k, 4), bar_init(xempty + 8 * k, 4);
+    for (int k = 0; k < NB; k++) bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 8);
+    for (int k = 0; k < 2; k++) bar_init(obar + 8 * k, 1), bar_init(xfull + 8 * k, 4), bar_init(xempty + 8 * k, 4);
     for (int k = 0; k < 8; k++) bar_init(hbar + 8 * k, 2);
     for (int k = 0; k < kRuns; k++) bar_init(rbar + 8 * k, 1);
     bar_init(dbar, 1);
-    bar_init(obar, 1);
     bar_init(endbar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     sh.fail = 0;
@@ -500,10 +505,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     return bar_wait(rbar + 8 * k, (r / kRuns) & 1, &sh.fail) ? &sh.runs[k] : nullptr;
   };
 
-  if (warp == kTaSoft) {
+  if (warp >= kTaSoft && warp < kTaSoft + kTaLoad) {
     // ------------------------------------------------------------ TMA
-    // tiles in the order the products use them: a pair of query tiles K0 V0 K1
-    // V1 ..., a single one K0 K1 V0 K2 V1 ...
+    const int part = warp - kTaSoft;
+    const bool lead = elect_one();
     uint32_t seq = 0, nr = 0;
     Walk<HD, Q> walk;
     walk.x0 = walk.x = share0;
@@ -511,7 +516,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     if (share0 < share1) walk.i = sh.req, walk.base = sh.base, walk.q = sh.q;
     Run run;
     auto hand_over = [&]() {
-      if (lane == 0) {
+      if (part == 0 && lane == 0) {
         sh.runs[nr % kRuns] = run;
         bar_arrive(rbar + 8 * (nr % kRuns));
       }
@@ -523,42 +528,52 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       hand_over();
       const int nt = run.nt;
       const int* table = a.tables + (size_t)run.i * a.ld_tables;
-      auto load = [&](const CUtensorMap* map, int tile) {
-        if (!ok) return;
-        const int pg = run.key0 / kKvPage + tile * PAGES + lane;
+      // first rows of the pages of 32 / PAGES tiles, a page per lane; the next
+      // batch is on its way while this one is used
+      auto fetch = [&](int batch) {
+        const int pg = run.key0 / kKvPage + batch * 32 + lane;
         int row = rows_end;
-        if (lane < PAGES && pg < a.max_pages && pg * kKvPage < run.keys) {
+        if (pg < a.max_pages && pg * kKvPage < run.keys) {
           const int id = table[pg];
           if (id >= 0 && id < a.n_pages) row = (id * a.kv_heads + run.kvh) * kKvPage;
         }
+        return row;
+      };
+      int before = rows_end, now = fetch(0), after = fetch(1), at = 0;
+      auto load = [&](const CUtensorMap* map, int tile) {
+        if (!ok) return;
+        const int batch = tile / (32 / PAGES);
+        if (batch > at) before = now, now = after, after = fetch(batch + 1), at = batch;
+        const int rows = batch == at ? now : before;  // V follows K by fewer tiles than a batch has
         const uint32_t slot = seq % NSLOT, bar = full + 8 * slot;
         if (seq >= NSLOT) ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * slot, (seq / NSLOT - 1) & 1, &sh.fail));
         if (!ok) return;
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"((uint32_t)S::kSlot)
+        if (lead)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar),
+                       "r"((uint32_t)(S::kSlot / kTaLoad))
                        : "memory");
-        __syncwarp();
-        if (lane < PAGES) {
 #pragma unroll
-          for (int h = 0; h < ATOMS; h++)
-            asm volatile(
-                "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-                "[%4];\n" ::"r"(ring + slot * S::kSlot + h * KT * 128 + lane * kKvPage * 128),
-                "l"(map), "r"(h * 64), "r"(row), "r"(bar)
-                : "memory");
+        for (int p = 0; p < PAGES / kTaLoad; p++) {
+          const int page = part * (PAGES / kTaLoad) + p;
+          const int row = __shfl_sync(0xffffffffu, rows, tile % (32 / PAGES) * PAGES + page);
+          if (lead) {
+#pragma unroll
+            for (int h = 0; h < ATOMS; h++)
+              asm volatile(
+                  "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+                  "[%4];\n" ::"r"(ring + slot * S::kSlot + h * KT * 128 + page * kKvPage * 128),
+                  "l"(map), "r"(h * 64), "r"(row), "r"(bar)
+                  : "memory");
+          }
         }
-        __syncwarp();
         seq++;
       };
-      if (run.w == 2) {
-        for (int t = 0; t < nt; t++) load(&mk, t), load(&mv, t);
-      } else {
-        load(&mk, 0);
-        if (nt > 1) load(&mk, 1);
-        for (int t = 0; t < nt; t++) {
-          load(&mv, t);
-          if (t + 2 < nt) load(&mk, t + 2);
-        }
+      // in the order the products use them: the K tiles whose scores run ahead, then V and K in turn
+      const int ahead = run.w == 2 ? NB / 2 : NB;
+      for (int t = 0; t < ahead && t < nt; t++) load(&mk, t);
+      for (int t = 0; t < nt; t++) {
+        load(&mv, t);
+        if (t + ahead < nt) load(&mk, t + ahead);
       }
     }
     run.nt = 0;
@@ -568,7 +583,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       int dummy = 0;
       bar_wait(full + 8 * (k % NSLOT), (k / NSLOT) & 1, &dummy);
     }
-  } else if (warp == kTaSoft + 1) {
+  } else if (warp == kTaSoft + kTaLoad) {
     // ------------------------------------------------------------ products
     // The whole warp follows the schedule, so that operands are formed in
     // uniform registers; one elected lane issues.  (With the loop run by a
@@ -576,7 +591,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     const bool lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     uint32_t seq = 0;          // tiles of the ring used up by earlier runs
-    uint32_t np[2] = {0, 0};   // P tiles taken from each buffer
+    uint32_t np = 0;           // parity of the P tiles taken from each buffer
     uint32_t runs = 0;
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -590,17 +605,18 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const bool pair = __shfl_sync(0xffffffffu, run->w, 0) == 2;
       if (nt == 0) break;
       const int nu = pair ? 2 * nt : nt;
-      // place in the ring's order of the K and V tile of unit u
-      auto k_at = [&](int u) { return pair ? (uint32_t)(u >> 1) * 2 : u < 2 ? (uint32_t)u : (uint32_t)(2 * u - 1); };
-      auto v_at = [&](int u) {
-        return pair ? (uint32_t)(u >> 1) * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt);
-      };
-      auto scores = [&](int u) {  // S[u % 2] = Q K^T
-        const uint32_t k = seq + k_at(u), slot = k % NSLOT;
+      // place in the ring's order of the K and V tile t
+      const int ahead = pair ? NB / 2 : NB;
+      auto k_at = [&](int t) { return (uint32_t)(t < ahead ? t : 2 * t - ahead + 1); };
+      auto v_at = [&](int t) { return (uint32_t)(min(nt, t + ahead) + t); };
+      // S buffer of unit u: streams take turns, each with two buffers
+      auto buf = [&](int u) { return NS == 2 ? (u & 1) * 2 + (u >> 1 & 1) : u & 1; };
+      auto scores = [&](int u) {  // S = Q K^T
+        const uint32_t k = seq + k_at(pair ? u >> 1 : u), slot = k % NSLOT;
         if (!wait(full + 8 * slot, (k / NSLOT) & 1)) return;
         fence_after();
         const uint32_t kb = desc_lo(ring + slot * S::kSlot, 16);
-        const uint32_t qb = desc_lo(qs + (pair ? (u & 1) * S::kQTile : 0), 16), d = tm + (u & 1) * KT;
+        const uint32_t qb = desc_lo(qs + (pair ? (u & 1) * S::kQTile : 0), 16), d = tm + buf(u) * KT;
         if (lead) {
 #pragma unroll
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
@@ -610,23 +626,23 @@ __global__ void __launch_bounds__(kTaThreads, 1)
               // that costs least while they are small
               mma_ss(d, qb + (((S::kSplit && !w ? NS * S::kQTile : 0) + (ks >> 2) * 128 * 128 + (ks & 3) * 32) >> 4),
                      kb + (((ks >> 2) * KT * 128 + (ks & 3) * 32) >> 4), S::kIdescS, w || ks ? 1u : 0u);
-          mma_commit(sbar + 8 * (u & 1));
+          mma_commit(sbar + 8 * buf(u));
           if (!pair || (u & 1)) mma_commit(empty + 8 * slot);
         }
       };
       if (!wait(qbar, runs & 1)) break;
       runs++;
       fence_after();
-      scores(0);
-      if (nu > 1) scores(1);
+      for (int u = 0; u < NB && u < nu; u++) scores(u);
       for (int u = 0; ok && u < nu; u++) {
-        const int b = u & 1;
-        const uint32_t k = seq + v_at(u), slot = k % NSLOT;
-        if (!wait(pbar + 8 * b, np[b]++ & 1) || !wait(full + 8 * slot, (k / NSLOT) & 1)) break;
+        const int b = buf(u), t = NS == 2 ? u & 1 : 0;
+        const uint32_t k = seq + v_at(pair ? u >> 1 : u), slot = k % NSLOT, parity = np >> b & 1;
+        np ^= 1u << b;
+        if (!wait(pbar + 8 * b, parity) || !wait(full + 8 * slot, (k / NSLOT) & 1)) break;
         fence_after();
         const uint32_t vb = desc_lo(ring + slot * S::kSlot, KT * 128);
-        const uint32_t d = tm + S::kO + (NS == 2 ? b * HD : 0), p = tm + b * KT;
-        const uint32_t acc = (NS == 2 ? u < 2 : u == 0) ? 0u : 1u;
+        const uint32_t d = tm + S::kO + t * HD, p = tm + b * KT;
+        const uint32_t acc = u < NS ? 0u : 1u;
         if (lead) {
 #pragma unroll
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
@@ -634,10 +650,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             for (int ks = 0; ks < KT / 16; ks++)
               mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8 + (S::kSplit && !w ? 16 : 0), vb + (ks * 16 * 128 >> 4),
                      S::kIdescO, w || ks ? 1u : acc);
-          if (!pair || b) mma_commit(empty + 8 * slot);
-          if (NS == 1) mma_commit(obar);
+          if (!pair || t) mma_commit(empty + 8 * slot);
+          mma_commit(obar + 8 * t);
         }
-        if (u + 2 < nu) scores(u + 2);
+        if (u + NB < nu) scores(u + NB);
       }
       if (!ok) break;
       if (lead) mma_commit(dbar);
@@ -658,7 +674,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     const uint32_t oth = hbar + 8 * (t * 4 + (warp & 3));  // meets the other half's warp
     const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0) + hf * OW;
     const float c = a.scale * 1.4426950408889634f;
-    uint32_t ns[2] = {0, 0}, runs = 0, no = 0, seq = 0;
+    uint32_t ns = 0, runs = 0, no = 0, seq = 0;  // ns: parities of the stream's two S buffers; no: its products so far
     uint32_t nx = 0;           // exchanges between the streams
     uint32_t nh = 0;           // and between the halves
     bool ok = true;
@@ -673,12 +689,13 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       arrive_warp(oth);
       ok = wait_warp(oth, nh++ & 1);
     };
-    // this row's value of the other half.  The next call writes over it: between
-    // two calls lie a product or a meet(), for which the other half has read.
+    // this row's value of the other half; the call after the next one writes
+    // over it, and lets this one's readers meet first
     auto swap_half = [&](float v) {
-      sh.half[t][hf][wt] = v;
+      const int k = nh & 1;
+      sh.half[k][NS == 2 ? t : 0][hf][wt] = v;
       meet();
-      return sh.half[t][hf ^ 1][wt];
+      return sh.half[k][NS == 2 ? t : 0][hf ^ 1][wt];
     };
     while (true) {
       const Run* rp = get_run(runs);
@@ -772,9 +789,11 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       };
       float mx = -INFINITY, l = 0.f;
       const int step = NS == 2 ? 2 : 1;
-      for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step) {
-        const int b = u & 1, tile = pair ? u >> 1 : u, key0 = first + tile * KT;
-        ok = wait_warp(sbar + 8 * b, ns[b]++ & 1);
+      for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step, no++) {
+        const int v = NS == 2 ? u >> 1 : u, b = (NS == 2 ? t * 2 : 0) + (v & 1);
+        const int tile = pair ? u >> 1 : u, key0 = first + tile * KT;
+        ok = wait_warp(sbar + 8 * b, ns >> (v & 1) & 1);
+        ns ^= 1u << (v & 1);
         if (!ok) break;
         fence_after();
         const uint32_t sp = tmem + lanes + b * KT + hf * CW;
@@ -782,32 +801,19 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           // which keys the row sees, when it is not all of them
           const bool plain = key0 + KT <= len && !holes && (a.window <= 0 || key0 > pos - a.window) && pos >= 0;
           const bool masked = !__all_sync(0xffffffffu, plain || !live);
-          uint32_t see[CW / 32];
+          uint32_t see = 0;
+          if (masked) see = visible(key0 + hf * CW);
+          __syncwarp();
+          float s[32], top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tm_ld32(sp, reinterpret_cast<uint32_t*>(s));
+          tm_wait_ld(reinterpret_cast<uint32_t*>(s));
           if (masked) {
 #pragma unroll
-            for (int k = 0; k < CW / 32; k++) see[k] = visible(key0 + hf * CW + 32 * k);
-            __syncwarp();
+            for (int e = 0; e < 32; e++) s[e] = see >> e & 1u ? s[e] : -INFINITY;
           }
-          // the scores come in 32 at a time, for the maximum and again for P:
-          // held in between, they would push the loop's state out of registers
-          float s[32], top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          auto load = [&](int k) {
-            tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
-            tm_wait_ld(reinterpret_cast<uint32_t*>(s));
-            if (masked) {
 #pragma unroll
-              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
-            }
-          };
-#pragma unroll
-          for (int k = 0; k < CW / 32; k++) {
-            load(k);
-#pragma unroll
-            for (int e = 0; e < 32; e++) top4[e & 3] = fmaxf(top4[e & 3], s[e]);
-          }
+          for (int e = 0; e < 32; e++) top4[e & 3] = fmaxf(top4[e & 3], s[e]);
           float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-          // with one stream the scores do not say that the last product is done
-          if (NS == 1 && u > 0 && !(ok = wait_warp(obar, no++ & 1))) break;
           top = fmaxf(top, swap_half(top)) * c;
           if (!ok) break;
           // follow the maximum; O and l are rescaled only past the lag
@@ -820,6 +826,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             l *= scale;
           }
           if (__any_sync(0xffffffffu, scale != 1.f)) {
+            // O is at rest once the stream's last product is done (the one before it is: these scores came after)
+            if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
             fence_after();
 #pragma unroll 1
             for (int k = 0; k < OW / 16; k++) {
@@ -833,34 +841,28 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          // over the scores they came from: 16 columns of high words, then low ones
 #pragma unroll
-          for (int k = 0; k < CW / 32; k++) {
-            if (CW > 32) load(k);
-            // over the scores they came from: 16 columns of high words, then low ones
+          for (int h = 0; h < 2; h++) {
+            uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              uint32_t hi[8], lo[8];
-#pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const float p0 = ex2(fmaf(s[16 * h + 2 * e], c, off)), p1 = ex2(fmaf(s[16 * h + 2 * e + 1], c, off));
-                sum[(2 * e) & 3] += p0;
-                sum[(2 * e + 1) & 3] += p1;
-                hi[e] = pack2(p0, p1, C());
-                if constexpr (S::kSplit) {
-                  __half2 x;
-                  memcpy(&x, &hi[e], 4);
-                  const float2 f = __half22float2(x);
-                  lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
-                }
+            for (int e = 0; e < 8; e++) {
+              const float p0 = ex2(fmaf(s[16 * h + 2 * e], c, off)), p1 = ex2(fmaf(s[16 * h + 2 * e + 1], c, off));
+              sum[(2 * e) & 3] += p0;
+              sum[(2 * e + 1) & 3] += p1;
+              hi[e] = pack2(p0, p1, C());
+              if constexpr (S::kSplit) {
+                __half2 x;
+                memcpy(&x, &hi[e], 4);
+                const float2 f = __half22float2(x);
+                lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
               }
-              tm_st8(sp + k * 32 + h * 8, hi);
-              if constexpr (S::kSplit) tm_st8(sp + k * 32 + 16 + h * 8, lo);
             }
+            tm_st8(sp + h * 8, hi);
+            if constexpr (S::kSplit) tm_st8(sp + 16 + h * 8, lo);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tm_wait_st();
-        } else if (NS == 1 && u > 0) {
-          no++;
         }
         if (hf == 0 && key0 + KT > len) {
           // V rows that no row sees: keys past the end, nodes in nobody's mask.
@@ -882,7 +884,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             }
             dead = key0 + wt >= run.keys || !(seen >> lane & 1u);
           }
-          const uint32_t k = seq + (pair ? (uint32_t)tile * 2 + 1 : (uint32_t)(u + 2 < nt ? 2 * u + 2 : u + nt));
+          const uint32_t k = seq + (uint32_t)(min(nt, tile + (pair ? NB / 2 : NB)) + tile);
           const uint32_t slot = k % NSLOT;
           ok = wait_warp(full + 8 * slot, (k / NSLOT) & 1);
           if (!ok) break;
@@ -903,7 +905,6 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (!ok) break;
       ok = wait_warp(dbar, runs++ & 1);
       if (!ok) break;
-      if (NS == 1) no++;  // the last product's phase
       fence_after();
       if (!(NS == 2 ? t < nu : t == 0)) continue;  // no tile for this stream
       l += swap_half(l);
@@ -913,7 +914,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       float own = 1.f, other = 0.f;
       if (merge && t == 1) {  // (m, l) for the other stream
         meet();
-        sh.half[1][hf][wt] = hf ? l : mx;
+        sh.half[0][NS - 1][hf][wt] = hf ? l : mx;
         if (ok) meet();
         if (!ok) break;
       }
@@ -942,7 +943,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           } else {
             if (!(ok = wait_warp(xfull + 8 * hf, nx & 1))) break;
             if (k == 0) {
-              const float2 ml = make_float2(sh.half[1][0][wt], sh.half[1][1][wt]);
+              const float2 ml = make_float2(sh.half[0][NS - 1][0][wt], sh.half[0][NS - 1][1][wt]);
               const float mn = fmaxf(mx, ml.x);
               own = l == 0.f ? 0.f : ex2(mx - mn);
               other = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
@@ -985,7 +986,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   }
   fence_before();
   __syncthreads();
-  if (warp == kTaSoft + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+  if (warp == kTaSoft + kTaLoad) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
   if (tid == 0) parts.status[blockIdx.x] = sh.fail;
 }
 
@@ -1104,7 +1105,7 @@ int launch_t(const TreeAttnArgs& a, cudaStream_t st) {
   WL_TRY(cache_map(&mv, a.cache_v, S::kBf16, HD, rows));
   const int ctas = device_sms();
   const Parts parts = parts_at(a.workspace, ctas, a.n, HD, part_rows(a.rows, a.heads / a.kv_heads));
-  constexpr int smem = kTaSmem + (int)sizeof(Small<S::kSlots>);
+  constexpr int smem = S::kTiles + (int)sizeof(Small<HD, Q>);
   if (first_use_on_device((const void*)k_tree_attn<HD, Q>))
     WL_CUDA_TRY(cudaFuncSetAttribute(k_tree_attn<HD, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   WL_TRY(launch_k(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
