@@ -22,11 +22,10 @@
 //   others     softmax, two threads per query row (half of a key tile's columns
 //              each): S from TMEM into registers, mask, running maximum and sum,
 //              P back over S.
-// They work on two streams, each with two S buffers, so that the scores run
-// ahead of the softmax and one stream's softmax under the other's products: the
-// two query tiles of a pair over the same keys or, for a single query tile,
-// even and odd key tiles, merged at the end.  head_dim 256 has room in TMEM for
-// one O only: one stream.
+// They work on two streams, so that one's softmax runs under the other's
+// products: the two query tiles of a pair over the same keys or, for a single
+// query tile, even and odd key tiles, merged at the end.  head_dim 256 has room
+// in TMEM for one O only: one stream, with two S buffers.
 // The maximum that P is taken against follows the true one with a lag of up to
 // 2^6 (O is rescaled only past that), and P is scaled by 2^8 where it is f16, so
 // that it stays clear of both ends of the type; both factors cancel in o / l.
@@ -143,13 +142,13 @@ constexpr int kTaLag = 6;             // log2 of the lag of the maximum
 template <int HD, class Q>
 struct Shape {
   static constexpr bool kSplit = sizeof(Q) == 4;       // f32 queries as two f16 words
-  static constexpr int KT = 64;                        // keys per tile
+  static constexpr int KT = HD == 256 ? 64 : 128;      // keys per tile
   static constexpr int NS = HD == 256 ? 1 : 2;         // streams
-  static constexpr int NB = 2 * NS;                    // S buffers, two per stream
+  static constexpr int NB = 2;                         // S buffers
   static constexpr int kQTile = 128 * HD * 2;          // bytes of a query tile (one word)
   static constexpr int kQBytes = kQTile * NS * (kSplit ? 2 : 1);
   static constexpr int kSlot = KT * HD * 2;            // bytes of a K or V tile
-  static constexpr int kFit = (kTaSmem - kQBytes - (NS == 2 ? 5376 : 3072)) / kSlot;
+  static constexpr int kFit = (kTaSmem - kQBytes - 3072) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
   static constexpr int kTiles = kQBytes + kSlots * kSlot;
   static constexpr int kO = 256;                       // TMEM column of O; S buffers from 0
@@ -257,6 +256,29 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
+}
+using f2 = unsigned long long;  // two f32 values, for the paired instructions
+__device__ __forceinline__ f2 make_f2(float x, float y) {
+  f2 v;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ float lo_of(f2 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(f2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ f2 fma2(f2 x, f2 y, f2 z) {
+  f2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+  return v;
+}
+__device__ __forceinline__ f2 add2(f2 x, f2 y) {
+  f2 v;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
+  return v;
 }
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -391,11 +413,11 @@ __device__ __forceinline__ void st4(float* p, const float* v) { *reinterpret_cas
 
 template <int HD, class Q>
 struct Small {  // behind the tiles in shared memory
-  static constexpr int NSLOT = Shape<HD, Q>::kSlots, NS = Shape<HD, Q>::NS;
+  static constexpr int NSLOT = Shape<HD, Q>::kSlots;
   uint64_t bars[2 * NSLOT + 26 + kRuns];
   Run runs[kRuns];
   union {
-    float half[2][NS][2][128];  // [parity of the exchange][stream][half][row]
+    float half[2][2][128];  // [stream][half][row]; one stream: [parity of the exchange]
     long long scan[kTaThreads / 32];  // at the start
   };
   long long base;
@@ -609,8 +631,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const int ahead = pair ? NB / 2 : NB;
       auto k_at = [&](int t) { return (uint32_t)(t < ahead ? t : 2 * t - ahead + 1); };
       auto v_at = [&](int t) { return (uint32_t)(min(nt, t + ahead) + t); };
-      // S buffer of unit u: streams take turns, each with two buffers
-      auto buf = [&](int u) { return NS == 2 ? (u & 1) * 2 + (u >> 1 & 1) : u & 1; };
+      // S buffer of unit u: one for each of two streams, or two for one
+      auto buf = [&](int u) { return u & 1; };
       auto scores = [&](int u) {  // S = Q K^T
         const uint32_t k = seq + k_at(pair ? u >> 1 : u), slot = k % NSLOT;
         if (!wait(full + 8 * slot, (k / NSLOT) & 1)) return;
@@ -674,7 +696,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     const uint32_t oth = hbar + 8 * (t * 4 + (warp & 3));  // meets the other half's warp
     const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0) + hf * OW;
     const float c = a.scale * 1.4426950408889634f;
-    uint32_t ns = 0, runs = 0, no = 0, seq = 0;  // ns: parities of the stream's two S buffers; no: its products so far
+    uint32_t ns = 0, runs = 0, no = 0, seq = 0;  // ns: parities of the stream's S buffers; no: its products so far
     uint32_t nx = 0;           // exchanges between the streams
     uint32_t nh = 0;           // and between the halves
     bool ok = true;
@@ -689,13 +711,14 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       arrive_warp(oth);
       ok = wait_warp(oth, nh++ & 1);
     };
-    // this row's value of the other half; the call after the next one writes
-    // over it, and lets this one's readers meet first
+    // this row's value of the other half.  It is written over by the next call
+    // (two streams: a product or a meet() lies between) or the one after that
+    // (one stream: whose readers the next call meets).
     auto swap_half = [&](float v) {
-      const int k = nh & 1;
-      sh.half[k][NS == 2 ? t : 0][hf][wt] = v;
+      const int k = NS == 2 ? t : nh & 1;
+      sh.half[k][hf][wt] = v;
       meet();
-      return sh.half[k][NS == 2 ? t : 0][hf ^ 1][wt];
+      return sh.half[k][hf ^ 1][wt];
     };
     while (true) {
       const Run* rp = get_run(runs);
@@ -787,33 +810,48 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         return see;
       };
+      // keys [open0, open1) are seen by all of the warp's rows
+      int open0 = live ? pos < 0 || holes ? INT_MAX : a.window > 0 ? pos - a.window + 1 : 0 : 0;
+      open0 = __reduce_max_sync(0xffffffffu, open0);
       float mx = -INFINITY, l = 0.f;
       const int step = NS == 2 ? 2 : 1;
       for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step, no++) {
-        const int v = NS == 2 ? u >> 1 : u, b = (NS == 2 ? t * 2 : 0) + (v & 1);
+        const int b = u & 1, v = NS == 2 ? 0 : b;
         const int tile = pair ? u >> 1 : u, key0 = first + tile * KT;
-        ok = wait_warp(sbar + 8 * b, ns >> (v & 1) & 1);
-        ns ^= 1u << (v & 1);
+        ok = wait_warp(sbar + 8 * b, ns >> v & 1);
+        ns ^= 1u << v;
         if (!ok) break;
         fence_after();
         const uint32_t sp = tmem + lanes + b * KT + hf * CW;
         if (warp_live) {
-          // which keys the row sees, when it is not all of them
-          const bool plain = key0 + KT <= len && !holes && (a.window <= 0 || key0 > pos - a.window) && pos >= 0;
-          const bool masked = !__all_sync(0xffffffffu, plain || !live);
-          uint32_t see = 0;
-          if (masked) see = visible(key0 + hf * CW);
-          __syncwarp();
-          float s[32], top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tm_ld32(sp, reinterpret_cast<uint32_t*>(s));
-          tm_wait_ld(reinterpret_cast<uint32_t*>(s));
+          // the scores, 32 at a time: for the maximum, and again for P (held in
+          // between, 64 of them push the loop's state out of registers)
+          const bool masked = key0 < open0 || key0 + KT > len;
+          uint32_t see[CW / 32];
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) s[e] = see >> e & 1u ? s[e] : -INFINITY;
+            for (int k = 0; k < CW / 32; k++) see[k] = visible(key0 + hf * CW + 32 * k);
+            __syncwarp();
           }
+          float s[32], top = -INFINITY;
+          auto load = [&](int k) {
+            tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
+            tm_wait_ld(reinterpret_cast<uint32_t*>(s));
+            if (masked) {
 #pragma unroll
-          for (int e = 0; e < 32; e++) top4[e & 3] = fmaxf(top4[e & 3], s[e]);
-          float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
+            }
+          };
+#pragma unroll
+          for (int k = 0; k < CW / 32; k++) {
+            load(k);
+            float t4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int e = 4; e < 32; e += 8)
+#pragma unroll
+              for (int x = 0; x < 4; x++) t4[x] = e + 4 < 32 ? max3(t4[x], s[e + x], s[e + 4 + x]) : fmaxf(t4[x], s[e + x]);
+            top = max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
+          }
           top = fmaxf(top, swap_half(top)) * c;
           if (!ok) break;
           // follow the maximum; O and l are rescaled only past the lag
@@ -840,28 +878,34 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             }
           }
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          // over the scores they came from: 16 columns of high words, then low ones
+          const f2 c2 = make_f2(c, c), off2 = make_f2(off, off);
+          f2 sum[2] = {make_f2(0.f, 0.f), make_f2(0.f, 0.f)};
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            uint32_t hi[8], lo[8];
+          for (int k = 0; k < CW / 32; k++) {
+            if (CW > 32) load(k);
+            // over the scores they came from: 16 columns of high words, then low ones
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float p0 = ex2(fmaf(s[16 * h + 2 * e], c, off)), p1 = ex2(fmaf(s[16 * h + 2 * e + 1], c, off));
-              sum[(2 * e) & 3] += p0;
-              sum[(2 * e + 1) & 3] += p1;
-              hi[e] = pack2(p0, p1, C());
-              if constexpr (S::kSplit) {
-                __half2 x;
-                memcpy(&x, &hi[e], 4);
-                const float2 f = __half22float2(x);
-                lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
+            for (int h = 0; h < 2; h++) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const f2 x = fma2(make_f2(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]), c2, off2);
+                const float p0 = ex2(lo_of(x)), p1 = ex2(hi_of(x));
+                sum[e & 1] = add2(sum[e & 1], make_f2(p0, p1));
+                hi[e] = pack2(p0, p1, C());
+                if constexpr (S::kSplit) {
+                  __half2 y;
+                  memcpy(&y, &hi[e], 4);
+                  const float2 f = __half22float2(y);
+                  lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
+                }
               }
+              tm_st8(sp + k * 32 + h * 8, hi);
+              if constexpr (S::kSplit) tm_st8(sp + k * 32 + 16 + h * 8, lo);
             }
-            tm_st8(sp + h * 8, hi);
-            if constexpr (S::kSplit) tm_st8(sp + 16 + h * 8, lo);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          sum[0] = add2(sum[0], sum[1]);
+          l += lo_of(sum[0]) + hi_of(sum[0]);
           tm_wait_st();
         }
         if (hf == 0 && key0 + KT > len) {
@@ -914,7 +958,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       float own = 1.f, other = 0.f;
       if (merge && t == 1) {  // (m, l) for the other stream
         meet();
-        sh.half[0][NS - 1][hf][wt] = hf ? l : mx;
+        sh.half[1][hf][wt] = hf ? l : mx;
         if (ok) meet();
         if (!ok) break;
       }
@@ -943,7 +987,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           } else {
             if (!(ok = wait_warp(xfull + 8 * hf, nx & 1))) break;
             if (k == 0) {
-              const float2 ml = make_float2(sh.half[0][NS - 1][0][wt], sh.half[0][NS - 1][1][wt]);
+              const float2 ml = make_float2(sh.half[1][0][wt], sh.half[1][1][wt]);
               const float mn = fmaxf(mx, ml.x);
               own = l == 0.f ? 0.f : ex2(mx - mn);
               other = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
