@@ -365,7 +365,7 @@ int append_t(const void* k, const void* v, size_t ldk, size_t ldv, const int* sl
   const size_t all = (size_t)rows * kvh * (hd / 8);
   const size_t blocks = ceil_div(all, 256);
   const int grid = (int)(blocks < 148 * 32 ? blocks : 148 * 32);
-  return launch_k(k_kv_append<S, C>, dim3(grid), dim3(256), 0, st, (const S*)k, (const S*)v, ldk, ldv, slots,
+  return launch_step(k_kv_append<S, C>, dim3(grid), dim3(256), 0, st, (const S*)k, (const S*)v, ldk, ldv, slots,
                   rows, kvh, hd, n_slots, (C*)ck, (C*)cv);
 }
 
@@ -375,13 +375,13 @@ int append_t(const void* k, const void* v, size_t ldk, size_t ldv, const int* sl
 // scatter takes a launch of its own over the whole GPU.
 int launch_block_tables(const PlanArgs& a, cudaStream_t st) {
   const bool one = a.rows <= kPlanThreads * 4;
-  WL_TRY(launch_k(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, one ? 1 : 0));
-  if (!one) WL_TRY(launch_k(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a));
+  WL_TRY(launch_step(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, one ? 1 : 0));
+  if (!one) WL_TRY(launch_step(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a));
   return WL_OK;
 }
 
 int launch_release_pages(const ReleaseArgs& a, cudaStream_t st) {
-  return launch_k(k_release, dim3(1), dim3(kPlanThreads), 0, st, a);
+  return launch_step(k_release, dim3(1), dim3(kPlanThreads), 0, st, a);
 }
 
 int launch_kv_append(int src, int cache, const void* k, const void* v, size_t ldk, size_t ldv, const int* slots,
@@ -400,7 +400,7 @@ int launch_kv_append(int src, int cache, const void* k, const void* v, size_t ld
 int launch_kv_commit(const int* tables, int ld_tables, int max_pages, const int* lengths, int n,
                      const int* accepted, const int* accepted_start, int total, int kvh, int hd, int n_pages,
                      void* ck, void* cv, cudaStream_t st) {
-  return launch_k(k_kv_commit, dim3(n, kvh), dim3(128), 0, st, tables, ld_tables, max_pages, lengths, accepted,
+  return launch_step(k_kv_commit, dim3(n, kvh), dim3(128), 0, st, tables, ld_tables, max_pages, lengths, accepted,
                   accepted_start, total, kvh, hd / 8, n_pages, (uint4*)ck, (uint4*)cv);
 }
 

@@ -46,4 +46,16 @@ int launch_k(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStr
   return WL_OK;
 }
 
+// launch_k with the attribute set whatever the thread's setting: for the
+// operators of a serving step, whose kernels all wait (pdl_wait) before they
+// touch global memory.  A launch then costs its set-up under the kernel before it.
+template <class... KArgs, class... Args>
+int launch_step(void (*kern)(KArgs...), Args&&... args) {
+  const bool was = pdl_enabled();
+  set_pdl(true);
+  const int s = launch_k(kern, std::forward<Args>(args)...);
+  set_pdl(was);
+  return s;
+}
+
 }  // namespace wl

@@ -15,12 +15,13 @@
 // cut evenly over one CTA per SM, whatever the lengths, each CTA finding its
 // share from a prefix sum over the requests.  A run that is not a whole group
 // leaves unnormalised parts (o, m, l), which k_tree_combine merges.
-//   two warps  bring K and V tiles in with TMA, a 16-token page at a time
+//   a warp     brings K and V tiles in with TMA, a 16-token page at a time
 //              (its 64-column halves land in 128-byte-swizzled rows);
-//   two warps  issue S = Q K^T into TMEM and O += P V (P from TMEM, V as the
+//   a warp     issues S = Q K^T into TMEM and O += P V (P from TMEM, V as the
 //              MN-major operand straight from its rows);
-//   others     softmax, a thread per query row: S from TMEM into registers, mask,
-//              running maximum and sum, P back over S.
+//   others     softmax, two threads per query row (half of a key tile's columns
+//              each): S from TMEM into registers, mask, running maximum and sum,
+//              P back over S.
 // They work on two streams, so that one's softmax runs under the other's
 // products: the two query tiles of a pair over the same keys or, for a single
 // query tile, even and odd key tiles, merged at the end.  head_dim 256 has room
@@ -132,10 +133,9 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
 
 
 // ---------------------------------------------------------------- tcgen05
-constexpr int kTaSoft = 8;           // softmax warps: 2 streams x 4 lane quarters
+constexpr int kTaSoft = 16;          // softmax warps: 2 streams x 2 halves of the key tile x 4 lane quarters
 constexpr int kTaLoad = 2;           // TMA warps, each with half of a tile's pages
-constexpr int kTaMma = kTaSoft + kTaLoad;  // two warps issue the products, one per stream
-constexpr int kTaThreads = (kTaMma + 2) * 32;
+constexpr int kTaThreads = (kTaSoft + kTaLoad + 1) * 32;
 constexpr int kTaSmem = 232448;      // a CTA's shared memory: query tiles, the ring of K / V tiles, Small
 constexpr int kTaLag = 6;             // log2 of the lag of the maximum
 
@@ -149,7 +149,7 @@ struct Shape {
   static constexpr int kQBytes = kQTile * NS * (kSplit ? 2 : 1);
   static constexpr int kSlot = KT * HD * 2;            // bytes of a K or V tile
   static constexpr int kFit = (kTaSmem - kQBytes - 3072) / kSlot;
-  static constexpr int kSlots = kFit < 10 ? kFit : 10;
+  static constexpr int kSlots = kFit < 12 ? kFit : 12;
   static constexpr int kTiles = kQBytes + kSlots * kSlot;
   static constexpr int kO = 256;                       // TMEM column of O; S buffers from 0
   static constexpr bool kBf16 = std::is_same<Q, __nv_bfloat16>::value;
@@ -232,6 +232,10 @@ __device__ __forceinline__ void tm_ld16(uint32_t a, uint32_t* v) {
       : WL_R8(v, 0), WL_R8(v, 8)
       : "r"(a));
 }
+__device__ __forceinline__ void tm_st8(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};\n" ::WL_I8(v, 0), "r"(a)
+               : "memory");
+}
 __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -275,32 +279,6 @@ __device__ __forceinline__ f2 add2(f2 x, f2 y) {
   f2 v;
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(x), "l"(y));
   return v;
-}
-constexpr float kE3[3] = {0.69328290f, 0.24221097f, 0.055008933f};
-constexpr float kE4[4] = {0.69312418f, 0.24024099f, 0.055906426f, 0.0095828530f};
-// 2^x for x <= 127, without the special-function unit: x = n + f with n the
-// nearest whole number (read off a sum with 1.5 * 2^23), a polynomial for 2^f on
-// [-1/2, 1/2] fitted to the least relative error with p(0) = 1 (degree 3: 1.0e-4,
-// degree 4: 3e-6), and n added to its exponent.  Below -127 the result is 0: at
-// x = -127 the polynomial gives 1, whose exponent field is then 0.
-template <int N>
-__device__ __forceinline__ f2 exp2_fma(f2 x) {
-  static_assert(N == 3 || N == 4, "degree");
-  constexpr float c1 = N == 3 ? kE3[0] : kE4[0], c2 = N == 3 ? kE3[1] : kE4[1], c3 = N == 3 ? kE3[2] : kE4[2];
-  x = make_f2(fmaxf(lo_of(x), -127.f), fmaxf(hi_of(x), -127.f));
-  const f2 t = add2(x, make_f2(12582912.f, 12582912.f));
-  const f2 n = add2(t, make_f2(-12582912.f, -12582912.f));
-  const f2 f = fma2(n, make_f2(-1.f, -1.f), x);
-  f2 p = make_f2(c3, c3);
-  if constexpr (N == 4) {
-    constexpr float c4 = kE4[3];
-    p = fma2(make_f2(c4, c4), f, p);
-  }
-  p = fma2(p, f, make_f2(c2, c2));
-  p = fma2(p, f, make_f2(c1, c1));
-  p = fma2(p, f, make_f2(1.f, 1.f));
-  const uint32_t a = (uint32_t)p + ((uint32_t)t << 23), b = (uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23);
-  return make_f2(__uint_as_float(a), __uint_as_float(b));
 }
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -360,7 +338,6 @@ struct Run {
   int nt;             // key tiles; 0: no further run
   int key0;           // first key
   int w;              // query tiles: 2, or 1
-  int rot;            // rows by which stream 1's copy of a single query tile is turned
   int len, keys;      // Req's
   int row0, T;
   int i, kvh, qt0;
@@ -368,7 +345,7 @@ struct Run {
 };
 // Runs in flight: the TMA warp is ahead by no more than the ring's tiles, two
 // or more to a run, the others by one run.
-constexpr int kRuns = 8;
+constexpr int kRuns = 10;
 
 // Walks the CTA's share [x, x1) of the laid-out key tiles; all threads alike.
 template <int HD, class Q>
@@ -394,9 +371,6 @@ struct Walk {
       const int ta = (int)((x - g0) >> (r.w - 1)), tb = (int)((e - g0) >> (r.w - 1));  // w is 1 or 2
       r.nt = tb - ta;
       r.key0 = (q.tile0 + ta) * S::KT;
-      // up to 64 rows: the second stream's lie in the other lane quarters, whose
-      // warps sit on the SM's other schedulers
-      r.rot = S::NS == 2 && r.w == 1 && (long long)q.T * (args.heads / args.kv_heads) - (long long)r.qt0 * 128 <= 64 ? 64 : 0;
       r.len = q.len, r.keys = q.keys, r.row0 = q.row0, r.T = q.T, r.i = i;
       r.first = x0 >= g0;
       r.whole = ta == 0 && tb == q.kt;
@@ -440,10 +414,13 @@ __device__ __forceinline__ void st4(float* p, const float* v) { *reinterpret_cas
 template <int HD, class Q>
 struct Small {  // behind the tiles in shared memory
   static constexpr int NSLOT = Shape<HD, Q>::kSlots;
-  uint64_t bars[3 * NSLOT + 12 + kRuns];
+  uint64_t bars[2 * NSLOT + 26 + kRuns];
   Run runs[kRuns];
-  float2 ml[128];  // (m, l) of the second stream's rows
-  long long scan[kTaThreads / 32], base;
+  union {
+    float half[2][2][128];  // [stream][half][row]; one stream: [parity of the exchange]
+    long long scan[kTaThreads / 32];  // at the start
+  };
+  long long base;
   Req q;
   int req, fail;
   uint32_t tmem;
@@ -465,28 +442,26 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     if (threadIdx.x == 0) parts.status[blockIdx.x] = 1;
     return;
   }
-  const uint32_t full = sptr(sh.bars), empty = full + 16 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
-                 pbar = sbar + 16, dbar = pbar + 16, obar = dbar + 8, endbar = obar + 16, xfull = endbar + 16,
-                 xempty = xfull + 8, rbar = xempty + 8;
+  const uint32_t full = sptr(sh.bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
+                 pbar = sbar + 32, dbar = pbar + 32, obar = dbar + 8, endbar = obar + 16, xfull = endbar + 8,
+                 xempty = xfull + 16, hbar = xempty + 16, rbar = hbar + 64;
   const uint32_t qs = sptr(sm), ring = qs + S::kQBytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.heads / a.kv_heads;
 
-  if (warp == kTaMma) {
+  if (warp == kTaSoft + kTaLoad) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sptr(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (tid == 0) {
-    for (int k = 0; k < 2 * NSLOT; k++) bar_init(full + 8 * k, kTaLoad);
-    for (int k = 0; k < NSLOT; k++) bar_init(empty + 8 * k, 2);
+    for (int k = 0; k < NSLOT; k++) bar_init(full + 8 * k, kTaLoad), bar_init(empty + 8 * k, 1);
     bar_init(qbar, kTaSoft);
-    for (int k = 0; k < 2; k++) bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 4), bar_init(obar + 8 * k, 1);
-    bar_init(xfull, 4);
-    bar_init(xempty, 4);
+    for (int k = 0; k < NB; k++) bar_init(sbar + 8 * k, 1), bar_init(pbar + 8 * k, 8);
+    for (int k = 0; k < 2; k++) bar_init(obar + 8 * k, 1), bar_init(xfull + 8 * k, 4), bar_init(xempty + 8 * k, 4);
+    for (int k = 0; k < 8; k++) bar_init(hbar + 8 * k, 2);
     for (int k = 0; k < kRuns; k++) bar_init(rbar + 8 * k, 1);
-    bar_init(dbar, 2);
+    bar_init(dbar, 1);
     bar_init(endbar, 1);
-    bar_init(endbar + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     sh.fail = 0;
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mk) : "memory");
@@ -546,13 +521,6 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
-  // Barrier of the ring's k-th tile: two per slot, used in turn.  The streams
-  // pass over each other's tiles, so one may come to a slot whose previous tile
-  // is still on its way; with a single barrier the parity that it waits for
-  // would then be that of the tile before, and let it through.
-  auto full_bar = [&](uint32_t k) { return full + 8 * (k % NSLOT + (k / NSLOT & 1) * NSLOT); };
-  auto full_parity = [&](uint32_t k) { return k / (2 * NSLOT) & 1; };
-
   // run r of the CTA, once the TMA warp has put it down; null when a wait gave up
   auto get_run = [&](uint32_t r) -> const Run* {
     const uint32_t k = r % kRuns;
@@ -599,7 +567,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         const int batch = tile / (32 / PAGES);
         if (batch > at) before = now, now = after, after = fetch(batch + 1), at = batch;
         const int rows = batch == at ? now : before;  // V follows K by fewer tiles than a batch has
-        const uint32_t slot = seq % NSLOT, bar = full_bar(seq);
+        const uint32_t slot = seq % NSLOT, bar = full + 8 * slot;
         if (seq >= NSLOT) ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * slot, (seq / NSLOT - 1) & 1, &sh.fail));
         if (!ok) return;
         if (lead)
@@ -635,19 +603,17 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     // every copy has landed before the CTA ends
     for (uint32_t k = seq > NSLOT ? seq - NSLOT : 0; k < seq; k++) {
       int dummy = 0;
-      bar_wait(full_bar(k), full_parity(k), &dummy);
+      bar_wait(full + 8 * (k % NSLOT), (k / NSLOT) & 1, &dummy);
     }
-  } else if (warp >= kTaMma) {
+  } else if (warp == kTaSoft + kTaLoad) {
     // ------------------------------------------------------------ products
-    // A warp per stream, so that one's waits lie under the other's products.
-    // The whole warp follows the schedule, which keeps operands in uniform
-    // registers; one elected lane issues.  (With the loop run by a single lane a
-    // product took about 90 cycles to issue.)
-    const int t = warp - kTaMma;
+    // The whole warp follows the schedule, so that operands are formed in
+    // uniform registers; one elected lane issues.  (With the loop run by a
+    // single lane a product took about 90 cycles to issue.)
     const bool lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    uint32_t seq = 0;   // tiles of the ring used up by earlier runs
-    uint32_t np = 0;    // parity of the P tiles taken from each S buffer
+    uint32_t seq = 0;          // tiles of the ring used up by earlier runs
+    uint32_t np = 0;           // parity of the P tiles taken from each buffer
     uint32_t runs = 0;
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -659,27 +625,20 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (!ok) break;
       const int nt = __shfl_sync(0xffffffffu, run->nt, 0);
       const bool pair = __shfl_sync(0xffffffffu, run->w, 0) == 2;
-      const bool two = pair || __shfl_sync(0xffffffffu, run->rot, 0);  // a query tile per stream
       if (nt == 0) break;
-      // place in the ring's order of the K and V tile i
+      const int nu = pair ? 2 * nt : nt;
+      // place in the ring's order of the K and V tile t
       const int ahead = pair ? NB / 2 : NB;
-      auto k_at = [&](int i) { return (uint32_t)(i < ahead ? i : 2 * i - ahead + 1); };
-      auto v_at = [&](int i) { return (uint32_t)(min(nt, i + ahead) + i); };
-      // the stream's tiles: all of a pair's, every second one, or all (one stream)
-      const int n = NS == 1 ? (t == 0 ? nt : 0) : pair ? nt : (nt + 1 - t) / 2;
-      auto tile = [&](int v) { return NS == 1 || pair ? v : 2 * v + t; };
-      auto buf = [&](int v) { return NS == 1 ? v & 1 : t; };
-      // a slot is free after an arrival for each stream; a tile that only one uses gets both from it
-      auto release = [&](uint32_t slot) {
-        mma_commit(empty + 8 * slot);
-        if (!pair) mma_commit(empty + 8 * slot);
-      };
-      auto scores = [&](int v) {  // S = Q K^T
-        const uint32_t k = seq + k_at(tile(v)), slot = k % NSLOT;
-        if (!wait(full_bar(k), full_parity(k))) return;
+      auto k_at = [&](int t) { return (uint32_t)(t < ahead ? t : 2 * t - ahead + 1); };
+      auto v_at = [&](int t) { return (uint32_t)(min(nt, t + ahead) + t); };
+      // S buffer of unit u: one for each of two streams, or two for one
+      auto buf = [&](int u) { return u & 1; };
+      auto scores = [&](int u) {  // S = Q K^T
+        const uint32_t k = seq + k_at(pair ? u >> 1 : u), slot = k % NSLOT;
+        if (!wait(full + 8 * slot, (k / NSLOT) & 1)) return;
         fence_after();
         const uint32_t kb = desc_lo(ring + slot * S::kSlot, 16);
-        const uint32_t qb = desc_lo(qs + (two ? t * S::kQTile : 0), 16), d = tm + buf(v) * KT;
+        const uint32_t qb = desc_lo(qs + (pair ? (u & 1) * S::kQTile : 0), 16), d = tm + buf(u) * KT;
         if (lead) {
 #pragma unroll
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
@@ -689,22 +648,23 @@ __global__ void __launch_bounds__(kTaThreads, 1)
               // that costs least while they are small
               mma_ss(d, qb + (((S::kSplit && !w ? NS * S::kQTile : 0) + (ks >> 2) * 128 * 128 + (ks & 3) * 32) >> 4),
                      kb + (((ks >> 2) * KT * 128 + (ks & 3) * 32) >> 4), S::kIdescS, w || ks ? 1u : 0u);
-          mma_commit(sbar + 8 * buf(v));
-          release(slot);
+          mma_commit(sbar + 8 * buf(u));
+          if (!pair || (u & 1)) mma_commit(empty + 8 * slot);
         }
       };
       if (!wait(qbar, runs & 1)) break;
       runs++;
       fence_after();
-      for (int v = 0; v < NB / NS && v < n; v++) scores(v);
-      for (int v = 0; ok && v < n; v++) {
-        const int b = buf(v);
-        const uint32_t k = seq + v_at(tile(v)), slot = k % NSLOT, parity = np >> b & 1;
+      for (int u = 0; u < NB && u < nu; u++) scores(u);
+      for (int u = 0; ok && u < nu; u++) {
+        const int b = buf(u), t = NS == 2 ? u & 1 : 0;
+        const uint32_t k = seq + v_at(pair ? u >> 1 : u), slot = k % NSLOT, parity = np >> b & 1;
         np ^= 1u << b;
-        if (!wait(full_bar(k), full_parity(k)) || !wait(pbar + 8 * b, parity)) break;
+        if (!wait(pbar + 8 * b, parity) || !wait(full + 8 * slot, (k / NSLOT) & 1)) break;
         fence_after();
         const uint32_t vb = desc_lo(ring + slot * S::kSlot, KT * 128);
-        const uint32_t d = tm + S::kO + t * HD, p = tm + b * KT, acc = v ? 1u : 0u;
+        const uint32_t d = tm + S::kO + t * HD, p = tm + b * KT;
+        const uint32_t acc = u < NS ? 0u : 1u;
         if (lead) {
 #pragma unroll
           for (int w = 0; w < (S::kSplit ? 2 : 1); w++)
@@ -712,29 +672,33 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             for (int ks = 0; ks < KT / 16; ks++)
               mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8 + (S::kSplit && !w ? 16 : 0), vb + (ks * 16 * 128 >> 4),
                      S::kIdescO, w || ks ? 1u : acc);
-          release(slot);
+          if (!pair || t) mma_commit(empty + 8 * slot);
           mma_commit(obar + 8 * t);
         }
-        if (v + NB / NS < n) scores(v + NB / NS);
+        if (u + NB < nu) scores(u + NB);
       }
       if (!ok) break;
       if (lead) mma_commit(dbar);
       seq += 2 * nt;
     }
     if (!ok && lead) {  // products in flight finish before TMEM is given back
-      mma_commit(endbar + 8 * t);
+      mma_commit(endbar);
       int dummy = 0;
-      bar_wait(endbar + 8 * t, 0, &dummy);
+      bar_wait(endbar, 0, &dummy);
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
-    const int t = warp >> 2, wt = (warp & 3) * 32 + lane;  // stream; row of its query tile
+    // stream t; half hf of the key tile's columns (and of O's); row wt of the query tile
+    const int t = warp >> 3, hf = (warp >> 2) & 1, wt = (warp & 3) * 32 + lane;
+    constexpr int CW = KT / 2, OW = HD / 2;  // columns of S and of O that a thread takes
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0);
+    const uint32_t oth = hbar + 8 * (t * 4 + (warp & 3));  // meets the other half's warp
+    const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0) + hf * OW;
     const float c = a.scale * 1.4426950408889634f;
     uint32_t ns = 0, runs = 0, no = 0, seq = 0;  // ns: parities of the stream's S buffers; no: its products so far
     uint32_t nx = 0;           // exchanges between the streams
+    uint32_t nh = 0;           // and between the halves
     bool ok = true;
     auto wait_warp = [&](uint32_t bar, uint32_t parity) {  // the same answer for the whole warp
       return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, &sh.fail));
@@ -743,11 +707,24 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       __syncwarp();
       if (lane == 0) bar_arrive(bar);
     };
+    auto meet = [&]() {
+      arrive_warp(oth);
+      ok = wait_warp(oth, nh++ & 1);
+    };
+    // this row's value of the other half.  It is written over by the next call
+    // (two streams: a product or a meet() lies between) or the one after that
+    // (one stream: whose readers the next call meets).
+    auto swap_half = [&](float v) {
+      const int k = NS == 2 ? t : nh & 1;
+      sh.half[k][hf][wt] = v;
+      meet();
+      return sh.half[k][hf ^ 1][wt];
+    };
     while (true) {
       const Run* rp = get_run(runs);
       if (!__all_sync(0xffffffffu, rp != nullptr) || rp->nt == 0) break;
       const Run& run = *rp;
-      const int nt = run.nt, pair = run.w == 2, nu = pair ? 2 * nt : nt, len = run.len, first = run.key0, rot = run.rot;
+      const int nt = run.nt, pair = run.w == 2, nu = pair ? 2 * nt : nt, len = run.len, first = run.key0;
       // queries: the threads copy 16-byte pieces of the (row, head) pairs
       {
         const int m0 = run.qt0 * 128, mn = min(run.w * 128, run.T * group - m0);
@@ -769,17 +746,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
               memcpy(&hi[k], &h, 4);
               lo[k] = pack2(f[2 * k] - __half2float(h0), f[2 * k + 1] - __half2float(h1), __half());
             }
-            const uint4 h4 = make_uint4(hi[0], hi[1], hi[2], hi[3]), l4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            *reinterpret_cast<uint4*>(d) = h4;
-            *reinterpret_cast<uint4*>(d + NS * S::kQTile) = l4;
-            if (rot) {
-              *reinterpret_cast<uint4*>(d + S::kQTile + 64 * 128) = h4;
-              *reinterpret_cast<uint4*>(d + S::kQTile + 64 * 128 + NS * S::kQTile) = l4;
-            }
+            *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(d + NS * S::kQTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            *reinterpret_cast<uint4*>(d) = v;
-            if (rot) *reinterpret_cast<uint4*>(d + S::kQTile + 64 * 128) = v;
+            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(p);
           }
         }
       }
@@ -787,8 +757,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       fence_before();
       arrive_warp(qbar);
 
-      const int wl = t ? wt ^ rot : wt;  // row of the query tile; rot is 64 or 0
-      const int m = (run.qt0 + (pair ? t : 0)) * 128 + wl;
+      const int m = (run.qt0 + (pair ? t : 0)) * 128 + wt;
       const int j = m / group, g = m - j * group;
       const bool live = m < run.T * group;
       const int row = run.row0 + (live ? j : 0);
@@ -853,129 +822,93 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         ns ^= 1u << v;
         if (!ok) break;
         fence_after();
-        const uint32_t sp = tmem + lanes + b * KT;
+        const uint32_t sp = tmem + lanes + b * KT + hf * CW;
         if (warp_live) {
+          // the scores, 32 at a time: for the maximum, and again for P (held in
+          // between, 64 of them push the loop's state out of registers)
           const bool masked = key0 < open0 || key0 + KT > len;
-          auto hide = [&](float (&s)[32], int k) {  // masked scores of chunk k
-            const uint32_t see = visible(key0 + 32 * k);
+          uint32_t see[CW / 32];
+          if (masked) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) s[e] = see >> e & 1u ? s[e] : -INFINITY;
+            for (int k = 0; k < CW / 32; k++) see[k] = visible(key0 + hf * CW + 32 * k);
             __syncwarp();
+          }
+          float s[32], top = -INFINITY;
+          auto load = [&](int k) {
+            tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
+            tm_wait_ld(reinterpret_cast<uint32_t*>(s));
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
+            }
           };
-          auto most = [&](const float (&s)[32], float top) {
+#pragma unroll
+          for (int k = 0; k < CW / 32; k++) {
+            load(k);
             float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int e = 4; e < 28; e += 8)
+            for (int e = 4; e < 32; e += 8)
 #pragma unroll
-              for (int x = 0; x < 4; x++) t4[x] = max3(t4[x], s[e + x], s[e + 4 + x]);
-#pragma unroll
-            for (int x = 0; x < 4; x++) t4[x] = fmaxf(t4[x], s[28 + x]);
-            return max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
-          };
-          float sum = 0.f;
-          // P is taken against the maximum as it stood.  Only when a row passes
-          // it by more than the lag (and on its first tile) the tile's own is
-          // found first, and O and l are rescaled; P waits in registers until
-          // that is known, so S is still there.  Split P does not fit there:
-          // it looks for the maximum every time.
-          bool look = S::kSplit || __any_sync(0xffffffffu, pos >= 0 && mx == -INFINITY);
-          while (true) {
-            if (look) {
-              float top = -INFINITY;
+              for (int x = 0; x < 4; x++) t4[x] = e + 4 < 32 ? max3(t4[x], s[e + x], s[e + 4 + x]) : fmaxf(t4[x], s[e + x]);
+            top = max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
+          }
+          top = fmaxf(top, swap_half(top)) * c;
+          if (!ok) break;
+          // follow the maximum; O and l are rescaled only past the lag
+          float scale = 1.f;
+          if (mx == -INFINITY) {
+            mx = top;
+          } else if (live && top > mx + kTaLag) {
+            scale = ex2(mx - top);
+            mx = top;
+            l *= scale;
+          }
+          if (__any_sync(0xffffffffu, scale != 1.f)) {
+            // O is at rest once the stream's last product is done (the one before it is: these scores came after)
+            if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
+            fence_after();
 #pragma unroll 1
-              for (int k = 0; k < KT / 32; k++) {
-                float s[32];
-                tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
-                tm_wait_ld(reinterpret_cast<uint32_t*>(s));
-                if (masked) hide(s, k);
-                top = most(s, top);
-              }
-              top *= c;
-              float scale = 1.f;
-              if (mx == -INFINITY) {
-                mx = top;
-              } else if (live && top > mx + kTaLag) {
-                scale = ex2(mx - top);
-                mx = top;
-                l *= scale;
-              }
-              if (__any_sync(0xffffffffu, scale != 1.f)) {
-                // O is at rest once the stream's last product is done
-                if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
-                fence_after();
-#pragma unroll 1
-                for (int k = 0; k < HD / 16; k++) {
-                  uint32_t v[16];
-                  tm_ld16(op + k * 16, v);
-                  tm_wait_ld16(v);
+            for (int k = 0; k < OW / 16; k++) {
+              uint32_t v[16];
+              tm_ld16(op + k * 16, v);
+              tm_wait_ld16(v);
 #pragma unroll
-                  for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
-                  tm_st16(op + k * 16, v);
-                }
-              }
+              for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
+              tm_st16(op + k * 16, v);
             }
-            const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
-            const f2 c2 = make_f2(c, c), off2 = make_f2(off, off);
-            f2 sum2[2] = {make_f2(0.f, 0.f), make_f2(0.f, 0.f)};
-            if constexpr (S::kSplit) {
-#pragma unroll 1
-              for (int k = 0; k < KT / 32; k++) {
-                float s[32];
-                tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
-                tm_wait_ld(reinterpret_cast<uint32_t*>(s));
-                if (masked) hide(s, k);
-                uint32_t hi[16], lo[16];
+          }
+          const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
+          const f2 c2 = make_f2(c, c), off2 = make_f2(off, off);
+          f2 sum[2] = {make_f2(0.f, 0.f), make_f2(0.f, 0.f)};
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                  const f2 x = fma2(make_f2(s[2 * e], s[2 * e + 1]), c2, off2);
-                  const float p0 = ex2(lo_of(x)), p1 = ex2(hi_of(x));
-                  sum2[e & 1] = add2(sum2[e & 1], make_f2(p0, p1));
-                  hi[e] = pack2(p0, p1, C());
+          for (int k = 0; k < CW / 32; k++) {
+            if (CW > 32) load(k);
+            // over the scores they came from: 16 columns of high words, then low ones
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const f2 x = fma2(make_f2(s[16 * h + 2 * e], s[16 * h + 2 * e + 1]), c2, off2);
+                const float p0 = ex2(lo_of(x)), p1 = ex2(hi_of(x));
+                sum[e & 1] = add2(sum[e & 1], make_f2(p0, p1));
+                hi[e] = pack2(p0, p1, C());
+                if constexpr (S::kSplit) {
                   __half2 y;
                   memcpy(&y, &hi[e], 4);
                   const float2 f = __half22float2(y);
                   lo[e] = pack2(p0 - f.x, p1 - f.y, __half());
                 }
-                // over the scores they came from: the high words, then the low ones
-                tm_st16(sp + k * 32, hi);
-                tm_st16(sp + k * 32 + 16, lo);
               }
-            } else {
-              uint32_t pk[KT / 2];
-              float s[2][32], top = -INFINITY;
-              tm_ld32(sp, reinterpret_cast<uint32_t*>(s[0]));
-#pragma unroll
-              for (int k = 0; k < KT / 32; k++) {
-                tm_wait_ld(reinterpret_cast<uint32_t*>(s[k & 1]));
-                if (k + 1 < KT / 32) tm_ld32(sp + (k + 1) * 32, reinterpret_cast<uint32_t*>(s[(k + 1) & 1]));
-                if (masked) hide(s[k & 1], k);
-                if (!look) top = most(s[k & 1], top);
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                  const f2 x = fma2(make_f2(s[k & 1][2 * e], s[k & 1][2 * e + 1]), c2, off2);
-                  // the special-function unit alone would set the pace: every
-                  // third pair goes through the FMA pipe
-                  const f2 y = e % 3 == 1 ? exp2_fma<S::kBf16 ? 3 : 4>(x) : make_f2(ex2(lo_of(x)), ex2(hi_of(x)));
-                  sum2[e & 1] = add2(sum2[e & 1], y);
-                  pk[k * 16 + e] = pack2(lo_of(y), hi_of(y), C());
-                }
-              }
-              if (!look && __any_sync(0xffffffffu, live && top * c > mx + kTaLag)) {
-                look = true;
-                continue;
-              }
-#pragma unroll
-              for (int k = 0; k < KT / 32; k++) tm_st16(sp + k * 32, pk + k * 16);
+              tm_st8(sp + k * 32 + h * 8, hi);
+              if constexpr (S::kSplit) tm_st8(sp + k * 32 + 16 + h * 8, lo);
             }
-            sum2[0] = add2(sum2[0], sum2[1]);
-            sum = lo_of(sum2[0]) + hi_of(sum2[0]);
-            break;
           }
-          if (!ok) break;
-          l += sum;
+          sum[0] = add2(sum[0], sum[1]);
+          l += lo_of(sum[0]) + hi_of(sum[0]);
           tm_wait_st();
         }
-        if (key0 + KT > len) {
+        if (hf == 0 && key0 + KT > len) {
           // V rows that no row sees: keys past the end, nodes in nobody's mask.
           // A warp takes 32 keys, its lanes the request's rows.
           const int k0 = key0 + (wt & ~31);
@@ -997,7 +930,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
           const uint32_t k = seq + (uint32_t)(min(nt, tile + (pair ? NB / 2 : NB)) + tile);
           const uint32_t slot = k % NSLOT;
-          ok = wait_warp(full_bar(k), full_parity(k));
+          ok = wait_warp(full + 8 * slot, (k / NSLOT) & 1);
           if (!ok) break;
           if (dead) {
             uint8_t* v = sm + S::kQBytes + slot * S::kSlot + wt * 128;
@@ -1018,20 +951,27 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (!ok) break;
       fence_after();
       if (!(NS == 2 ? t < nu : t == 0)) continue;  // no tile for this stream
+      l += swap_half(l);
+      if (!ok) break;
       const bool merge = NS == 2 && run.whole && !pair && nu > 1;  // two streams of one row, joined here
-      float* xb = reinterpret_cast<float*>(sm + S::kQTile);  // [16][128]: the second query tile's place is free
+      float* xb = reinterpret_cast<float*>(sm + S::kQTile) + hf * 16 * 128;  // the second query tile's place is free
       float own = 1.f, other = 0.f;
-      if (merge && t == 1) sh.ml[wl] = make_float2(mx, l);
-      float* po = nullptr;
-      if (!run.whole && live && wl < parts.prow) {
-        const size_t at = (((size_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * 2 + t) * parts.prow + wl;
-        po = parts.o + at * HD;
-        *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(mx, l);
+      if (merge && t == 1) {  // (m, l) for the other stream
+        meet();
+        sh.half[1][hf][wt] = hf ? l : mx;
+        if (ok) meet();
+        if (!ok) break;
       }
-      Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD;
+      float* po = nullptr;
+      if (!run.whole && live && wt < parts.prow) {
+        const size_t at = (((size_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * 2 + t) * parts.prow + wt;
+        po = parts.o + at * HD + hf * OW;
+        if (hf == 0) *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(mx, l);
+      }
+      Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD + hf * OW;
       const bool write = run.whole && live && !(merge && t == 1);
 #pragma unroll 1
-      for (int k = 0; k < HD / 16; k++) {
+      for (int k = 0; k < OW / 16; k++) {
         float v[16];
         __syncwarp();
         if (warp_live) {
@@ -1040,14 +980,14 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         if (merge) {
           if (t == 1) {
-            if (nx > 0 && !(ok = wait_warp(xempty, (nx - 1) & 1))) break;
+            if (nx > 0 && !(ok = wait_warp(xempty + 8 * hf, (nx - 1) & 1))) break;
 #pragma unroll
-            for (int e = 0; e < 16; e++) xb[e * 128 + wl] = v[e];
-            arrive_warp(xfull);
+            for (int e = 0; e < 16; e++) xb[e * 128 + wt] = v[e];
+            arrive_warp(xfull + 8 * hf);
           } else {
-            if (!(ok = wait_warp(xfull, nx & 1))) break;
+            if (!(ok = wait_warp(xfull + 8 * hf, nx & 1))) break;
             if (k == 0) {
-              const float2 ml = sh.ml[wt];
+              const float2 ml = make_float2(sh.half[1][0][wt], sh.half[1][1][wt]);
               const float mn = fmaxf(mx, ml.x);
               own = l == 0.f ? 0.f : ex2(mx - mn);
               other = ml.y == 0.f ? 0.f : ex2(ml.x - mn);
@@ -1055,7 +995,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             }
 #pragma unroll
             for (int e = 0; e < 16; e++) v[e] = v[e] * own + xb[e * 128 + wt] * other;
-            arrive_warp(xempty);
+            arrive_warp(xempty + 8 * hf);
           }
           nx++;
         }
@@ -1085,12 +1025,12 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
       }
       // the exchange's last round has been read before its place is written again
-      if (merge && t == 1 && ok) ok = wait_warp(xempty, (nx - 1) & 1);
+      if (merge && t == 1 && ok) ok = wait_warp(xempty + 8 * hf, (nx - 1) & 1);
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == kTaMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+  if (warp == kTaSoft + kTaLoad) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
   if (tid == 0) parts.status[blockIdx.x] = sh.fail;
 }
 
@@ -1103,6 +1043,7 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
   const int lane = threadIdx.x & 31, r = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
   const int group = a.heads / a.kv_heads;
   pdl_wait();
+  pdl_trigger();
   if (head >= a.heads || r >= min(a.row_start[a.n], a.rows)) return;
   const long long per = parts.start[a.n + 1];
   bool failed = false;
@@ -1212,13 +1153,8 @@ int launch_t(const TreeAttnArgs& a, cudaStream_t st) {
   constexpr int smem = S::kTiles + (int)sizeof(Small<HD, Q>);
   if (first_use_on_device((const void*)k_tree_attn<HD, Q>))
     WL_CUDA_TRY(cudaFuncSetAttribute(k_tree_attn<HD, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  WL_TRY(launch_k(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
-  // the merge is launched under the main kernel and waits for its end
-  const bool was = pdl_enabled();
-  set_pdl(true);
-  const int e = launch_k(k_tree_combine<HD, Q>, dim3(a.rows, (a.heads + 3) / 4), dim3(128), 0, st, a, parts, ctas);
-  set_pdl(was);
-  return e;
+  WL_TRY(launch_step(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
+  return launch_step(k_tree_combine<HD, Q>, dim3(a.rows, (a.heads + 3) / 4), dim3(128), 0, st, a, parts, ctas);
 }
 
 template <class Q, class C>
@@ -1228,7 +1164,7 @@ int launch_hd(const TreeAttnArgs& a, cudaStream_t st) {
     case 128: return launch_t<128, Q>(a, st);
     case 256: return launch_t<256, Q>(a, st);
   }
-  return launch_k(k_tree_attn_row<Q, C>, dim3(a.rows, a.heads), dim3(128), 0, st, a);
+  return launch_step(k_tree_attn_row<Q, C>, dim3(a.rows, a.heads), dim3(128), 0, st, a);
 }
 
 }  // namespace
