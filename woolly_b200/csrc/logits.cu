@@ -10,13 +10,20 @@
 //   y = -inf                                         if the row's mask has bit v clear
 // in f32, rounded once to the logits' type.
 //
-// One CTA takes a run of the vocabulary of one row or, when the rows are drafts
-// of the same requests, of several: a word of shared memory per token counts its
-// occurrences (top bits: seen in the prompt, has a bias), a second one holds the
-// last bias entry that names it.  The history is counted once for the rows that
-// share it; a row's path and biases are put in before its run streams through,
-// four tokens at a time, and taken out after it.  The counts are integers and the
-// entry a maximum, so atomics' order is not seen.
+// Most tokens of a row are open and unseen: they are copied, or closed, in one
+// pass over the row that asks for nothing but the mask.  The others are few.  One
+// CTA takes a run of the vocabulary of one row or, when the rows are drafts of the
+// same requests, of eight: a word of shared memory per token counts its
+// occurrences in the history (top bit: seen in the prompt), once for the rows that
+// share it, and whoever turns a token's word from zero puts the token on a list.
+// The tokens of each row's path and its biases that fall into the run make a
+// second, short list.  Then a thread per (row, listed token) works out its value
+// from the logit that the copy left in place, adding what the row's short list has
+// to say about it; all rows of a request at once, so that the few dependent loads
+// are paid once and not row by row.  A row whose short list does not fit marks its
+// tokens in shared memory instead, and goes by itself.
+// Counts are integers and of a token's biases the last holds, so atomics' order is
+// not seen.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -33,7 +40,9 @@ namespace {
 
 constexpr int kLT = 512;        // threads
 constexpr int kLChunk = 4096;   // tokens of the vocabulary per CTA
-constexpr unsigned kPrompt = 0x80000000u, kBias = 0x40000000u;
+constexpr int kLRows = 8;       // most rows per CTA
+constexpr int kLOwn = 64;       // path and bias tokens of a row that its list holds
+constexpr unsigned kPrompt = 0x80000000u;
 
 __device__ __forceinline__ float get(const float* p) { return *p; }
 __device__ __forceinline__ float get(const __half* p) { return __half2float(*p); }
@@ -68,142 +77,224 @@ __device__ __forceinline__ void put4(T* p, const float* f) {
 
 // VEC: every row of four values is aligned
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kLT) k_logits(const LogitArgs a, int per) {
+__global__ void __launch_bounds__(kLT, 2) k_logits(const LogitArgs a, int per) {
   __shared__ __align__(16) unsigned seen[kLChunk];
   __shared__ __align__(16) int entry[kLChunk];
+  __shared__ unsigned short list[kLChunk];
+  __shared__ int s_req[kLRows], s_first[kLRows], s_b0[kLRows], s_b1[kLRows];
+  __shared__ wl_logit_params s_prm[kLRows];
+  __shared__ int2 own[kLRows][kLOwn];  // (token, bias entry, or -1 for a node of the path)
+  __shared__ int s_own[kLRows];        // how many there are
+  __shared__ int s_n;                  // listed tokens
   constexpr int NV = kLChunk / kLT;  // tokens per thread
   const int tid = threadIdx.x, v0 = blockIdx.y * kLChunk, nv = min(kLChunk, a.vocab - v0);
-  const int r0 = blockIdx.x * per, r1 = min(a.rows, r0 + per);
+  const int r0 = blockIdx.x * per, nr = min(per, a.rows - r0);
   pdl_wait();
   pdl_trigger();
   const wl_logit_context& c = a.ctx;
-  // first token of the thread's g-th group of four (VEC), or its g-th token
-  auto at = [&](int g) { return VEC ? (g * kLT + tid) * 4 : g * kLT + tid; };
   for (int i = tid * 4; i < kLChunk; i += kLT * 4) {
     *reinterpret_cast<uint4*>(seen + i) = make_uint4(0, 0, 0, 0);
     *reinterpret_cast<int4*>(entry + i) = make_int4(-1, -1, -1, -1);
   }
-  int counted = -1;  // the request whose history `seen` holds
-  for (int r = r0; r < r1; r++) {
-    const wl_logit_params p = a.params[r];
-    const T* x = (const T*)a.logits + (size_t)r * a.ld + v0;
-    T* y = (T*)a.out + (size_t)r * a.ldo + v0;
-    float f[NV];  // the row's logits are on their way while the counts are made
-    if constexpr (VEC) {
-#pragma unroll
-      for (int g = 0; g < NV / 4; g++)
-        if (at(g) + 4 <= nv) get4(x + at(g), f + 4 * g);
-        else
-          for (int e = 0; e < 4; e++) f[4 * g + e] = at(g) + e < nv ? get(x + at(g) + e) : 0.f;
-    } else {
-#pragma unroll
-      for (int g = 0; g < NV; g++) f[g] = at(g) < nv ? get(x + at(g)) : 0.f;
-    }
-    int b0 = 0, b1 = 0;
-    if (c.bias_start) {
-      b0 = min(max(c.bias_start[r], 0), c.bias_total);
-      b1 = min(max(c.bias_start[r + 1], 0), c.bias_total);
-    }
-    const int req = c.requests ? c.requests[r] : r;
+  if (tid == 0) s_n = 0;
+  if (tid < nr) {
+    const int r = r0 + tid, req = c.requests ? c.requests[r] : r;
     const bool has = req >= 0 && req < c.n_history;
-    if (r == r0 || req != counted) {
-      if (r != r0)
-        for (int i = tid * 4; i < kLChunk; i += kLT * 4) *reinterpret_cast<uint4*>(seen + i) = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-      counted = req;
-      if (has && c.history_start) {
-        const int h0 = min(max(c.history_start[req], 0), c.history_total);
-        const int h1 = min(max(c.history_start[req + 1], 0), c.history_total);
-        const int np = c.prompt_lens ? c.prompt_lens[req] : 0;
-#pragma unroll 4
-        for (int h = h0 + tid; h < h1; h += kLT) {
-          const unsigned v = (unsigned)c.history[h] - (unsigned)v0;
-          if (v >= (unsigned)nv) continue;
-          if (h - h0 < np) atomicOr(&seen[v], kPrompt);
-          else atomicAdd(&seen[v], 1u);
-        }
-      }
-    }
-    // the row's own tokens and biases: put in (add = 1), or taken out again
-    auto own = [&](bool add) {
-      if (has && c.draft_mask) {
-        const int row0 = c.row_start[req];
-        for (int d = tid; d < 32 * c.words; d += kLT) {
-          if (!(c.draft_mask[(size_t)r * c.words + (d >> 5)] >> (d & 31) & 1u)) continue;
-          if (row0 < 0 || row0 + d >= a.rows) continue;
-          const unsigned v = (unsigned)c.draft_tokens[row0 + d] - (unsigned)v0;
-          if (v < (unsigned)nv) atomicAdd(&seen[v], add ? 1u : ~0u);
-        }
-      }
-      for (int b = b0 + tid; b < b1; b += kLT) {
-        const unsigned v = (unsigned)c.bias_tokens[b] - (unsigned)v0;
-        if (v >= (unsigned)nv) continue;
-        if (add) {
-          atomicMax(&entry[v], b);
-          atomicOr(&seen[v], kBias);
-        } else {
-          entry[v] = -1;
-          atomicAnd(&seen[v], ~kBias);
-        }
-      }
-    };
-    own(true);
-    const unsigned* open = nullptr;
-    if (c.allowed && p.allowed_row >= 0 && p.allowed_row < c.n_allowed)
-      open = c.allowed + (size_t)p.allowed_row * c.allowed_words;
-    __syncthreads();
-    auto rules = [&](float x, unsigned s, int v) {
-      if (s & ~kBias) {
-        x = x > 0.f ? x / p.repetition : x * p.repetition;
-        const unsigned made = s & ~(kPrompt | kBias);
-        if (made) x -= p.frequency * (float)made + p.presence;
-      }
-      if (s & kBias) x += c.bias_values[entry[v]];
-      return x;
-    };
-    if constexpr (VEC) {
+    s_prm[tid] = a.params[r];
+    s_req[tid] = has ? req : -1;
+    s_own[tid] = 0;
+    s_first[tid] = has && c.draft_mask ? c.row_start[req] : -1;
+    s_b0[tid] = c.bias_start ? min(max(c.bias_start[r], 0), c.bias_total) : 0;
+    s_b1[tid] = c.bias_start ? min(max(c.bias_start[r + 1], 0), c.bias_total) : 0;
+  }
+  __syncthreads();
+  auto mask_of = [&](int k) {
+    const int m = s_prm[k].allowed_row;
+    return c.allowed && m >= 0 && m < c.n_allowed ? c.allowed + (size_t)m * c.allowed_words : nullptr;
+  };
+
+  // the copy; its loads run ahead of its stores by four rows
+  if constexpr (VEC) {
+    constexpr int G = NV / 4;
+    const int at = tid * 4;
+    float f0[NV], f1[NV], f2[NV], f3[NV];
+    auto load = [&](int k, float (&q)[NV]) {
+      if (k >= nr) return;
+      const T* x = (const T*)a.logits + (size_t)(r0 + k) * a.ld + v0;
 #pragma unroll
-      for (int g = 0; g < NV / 4; g++) {
-        const int v = at(g);
-        if (v >= nv) continue;
-        const uint4 s = *reinterpret_cast<const uint4*>(seen + v);
-        float* q = f + 4 * g;
-        if (s.x | s.y | s.z | s.w) {
-          q[0] = rules(q[0], s.x, v), q[1] = rules(q[1], s.y, v + 1);
-          q[2] = rules(q[2], s.z, v + 2), q[3] = rules(q[3], s.w, v + 3);
+      for (int g = 0; g < G; g++) {
+        const int v = at + g * kLT * 4;
+        if (v + 4 <= nv) {
+          get4(x + v, q + 4 * g);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) q[4 * g + e] = v + e < nv ? get(x + v + e) : 0.f;
         }
+      }
+    };
+    auto store = [&](int k, float (&q)[NV]) {
+      if (k >= nr) return;
+      const unsigned* open = mask_of(k);
+      T* y = (T*)a.out + (size_t)(r0 + k) * a.ldo + v0;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int v = at + g * kLT * 4;
+        if (v >= nv) continue;
         if (open) {
           const unsigned bits = open[(v0 + v) >> 5] >> ((v0 + v) & 31);
 #pragma unroll
-          for (int e = 0; e < 4; e++) q[e] = bits >> e & 1u ? q[e] : -INFINITY;
+          for (int e = 0; e < 4; e++) q[4 * g + e] = bits >> e & 1u ? q[4 * g + e] : -INFINITY;
         }
-        if (v + 4 <= nv) put4(y + v, q);
-        else
-          for (int e = 0; v + e < nv; e++) put(y + v + e, q[e]);
+        if (v + 4 <= nv) {
+          put4(y + v, q + 4 * g);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (v + e < nv) put(y + v + e, q[4 * g + e]);
+        }
       }
-    } else {
+    };
+    load(0, f0), load(1, f1), load(2, f2), load(3, f3);
+#pragma unroll 1
+    for (int k = 0; k < nr; k += 4) {
+      store(k, f0), load(k + 4, f0);
+      store(k + 1, f1), load(k + 5, f1);
+      store(k + 2, f2), load(k + 6, f2);
+      store(k + 3, f3), load(k + 7, f3);
+    }
+  } else {
+    for (int k = 0; k < nr; k++) {
+      const unsigned* open = mask_of(k);
+      const T* x = (const T*)a.logits + (size_t)(r0 + k) * a.ld + v0;
+      T* y = (T*)a.out + (size_t)(r0 + k) * a.ldo + v0;
+      float f[NV];
+#pragma unroll
+      for (int g = 0; g < NV; g++) f[g] = g * kLT + tid < nv ? get(x + g * kLT + tid) : 0.f;
 #pragma unroll
       for (int g = 0; g < NV; g++) {
-        const int v = at(g);
+        const int v = g * kLT + tid;
         if (v >= nv) continue;
-        const unsigned s = seen[v];
-        float z = s ? rules(f[g], s, v) : f[g];
-        if (open && !(open[(v0 + v) >> 5] >> ((v0 + v) & 31) & 1u)) z = -INFINITY;
-        put(y + v, z);
+        put(y + v, open && !(open[(v0 + v) >> 5] >> ((v0 + v) & 31) & 1u) ? -INFINITY : f[g]);
       }
     }
-    if (r + 1 < r1) {
+  }
+
+  // the rows' own tokens that fall into this run, kLT / per threads to a row
+  {
+    const int k = tid / (kLT / per), t = tid % (kLT / per);
+    auto note = [&](unsigned token, int b) {
+      const unsigned v = token - (unsigned)v0;
+      if (v >= (unsigned)nv) return;
+      const int e = atomicAdd(&s_own[k], 1);
+      if (e < kLOwn) own[k][e] = make_int2((int)v, b);
+    };
+    if (k < nr) {
+      const int row0 = s_first[k];
+      if (row0 >= 0)
+        for (int d = t; d < 32 * c.words && d < a.rows - row0; d += kLT / per)
+          if (c.draft_mask[(size_t)(r0 + k) * c.words + (d >> 5)] >> (d & 31) & 1u) note(c.draft_tokens[row0 + d], -1);
+#pragma unroll 4
+      for (int b = s_b0[k] + t; b < s_b1[k]; b += kLT / per) note(c.bias_tokens[b], b);
+    }
+  }
+  // seen: word of the token, made: times on the row's path, b: its bias entry
+  auto apply = [&](int k, int v, unsigned w, unsigned made, int b) {
+    const wl_logit_params& p = s_prm[k];
+    const unsigned* open = mask_of(k);
+    if (open && !(open[(v0 + v) >> 5] >> ((v0 + v) & 31) & 1u)) return;
+    T* y = (T*)a.out + (size_t)(r0 + k) * a.ldo + v0 + v;
+    float z = get(y);
+    made += w & ~kPrompt;
+    if (w | made) z = z > 0.f ? z / p.repetition : z * p.repetition;
+    if (made) z -= p.frequency * (float)made + p.presence;
+    if (b >= 0) z += c.bias_values[b];
+    put(y, z);
+  };
+  for (int k0 = 0, k1; k0 < nr; k0 = k1) {
+    const int req = s_req[k0];
+    for (k1 = k0 + 1; k1 < nr && s_req[k1] == req; k1++) {
+    }
+    if (k0 > 0) {  // another history
       __syncthreads();
-      own(false);
+      for (int i = tid * 4; i < kLChunk; i += kLT * 4) *reinterpret_cast<uint4*>(seen + i) = make_uint4(0, 0, 0, 0);
+      if (tid == 0) s_n = 0;
       __syncthreads();
+    }
+    if (req >= 0 && c.history_start) {
+      const int h0 = min(max(c.history_start[req], 0), c.history_total);
+      const int h1 = min(max(c.history_start[req + 1], 0), c.history_total);
+      const int np = c.prompt_lens ? c.prompt_lens[req] : 0;
+#pragma unroll 4
+      for (int h = h0 + tid; h < h1; h += kLT) {
+        const unsigned v = (unsigned)c.history[h] - (unsigned)v0;
+        if (v >= (unsigned)nv) continue;
+        const unsigned was = h - h0 < np ? atomicOr(&seen[v], kPrompt) : atomicAdd(&seen[v], 1u);
+        if (was == 0) list[atomicAdd(&s_n, 1)] = (unsigned short)v;
+      }
+    }
+    __syncthreads();  // the list, the rows' own and their copies are complete
+    const int n = s_n;
+    for (int i = tid; i < n * (k1 - k0); i += kLT) {
+      const int k = k0 + i / n, v = list[i % n], m = s_own[k];
+      if (m > kLOwn) continue;
+      unsigned made = 0;
+      int b = -1;
+      for (int e = 0; e < m; e++)
+        if (own[k][e].x == v) {
+          made += own[k][e].y < 0;
+          b = max(b, own[k][e].y);
+        }
+      apply(k, v, seen[v], made, b);
+    }
+    // own tokens that the history does not have: the first of several speaks for the token
+    for (int i = tid; i < kLOwn * (k1 - k0); i += kLT) {
+      const int k = k0 + i / kLOwn, j = i % kLOwn, m = s_own[k];
+      if (m > kLOwn || j >= m) continue;
+      const int v = own[k][j].x;
+      bool mine = seen[v] == 0;
+      unsigned made = 0;
+      int b = -1;
+      for (int e = 0; e < m && mine; e++)
+        if (own[k][e].x == v) {
+          mine = e >= j;
+          made += own[k][e].y < 0;
+          b = max(b, own[k][e].y);
+        }
+      if (mine) apply(k, v, 0, made, b);
+    }
+    for (int k = k0; k < k1; k++) {
+      if (s_own[k] <= kLOwn) continue;
+      // marks: path counts go into the words, the last bias entry beside them
+      const int row0 = s_first[k];
+      auto marks = [&](bool add) {
+        if (row0 >= 0)
+          for (int d = tid; d < 32 * c.words && d < a.rows - row0; d += kLT) {
+            if (!(c.draft_mask[(size_t)(r0 + k) * c.words + (d >> 5)] >> (d & 31) & 1u)) continue;
+            const unsigned v = (unsigned)c.draft_tokens[row0 + d] - (unsigned)v0;
+            if (v < (unsigned)nv) atomicAdd(&seen[v], add ? 1u : ~0u);
+          }
+        for (int b = s_b0[k] + tid; b < s_b1[k]; b += kLT) {
+          const unsigned v = (unsigned)c.bias_tokens[b] - (unsigned)v0;
+          if (v >= (unsigned)nv) continue;
+          if (add) atomicMax(&entry[v], b);
+          else entry[v] = -1;
+        }
+      };
+      __syncthreads();  // every reader of the words is done
+      marks(true);
+      __syncthreads();
+      for (int v = tid; v < nv; v += kLT)
+        if (seen[v] || entry[v] >= 0) apply(k, v, seen[v], 0, entry[v]);
+      __syncthreads();
+      marks(false);
     }
   }
 }
 
 template <class T>
 int launch_t(const LogitArgs& a, cudaStream_t st) {
-  // drafted rows share their request's history: eight at a time count it once
-  const int per = a.ctx.draft_mask ? 8 : 1;
+  // drafted rows share their request's history: a CTA counts it once for eight
+  const int per = a.ctx.draft_mask ? kLRows : 1;
   const dim3 grid((a.rows + per - 1) / per, (a.vocab + kLChunk - 1) / kLChunk);
   const size_t step = 4 * sizeof(T);
   const bool vec = !((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.out) |

@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanRows = 4096;  // rows that the scan's CTA places itself
 
 __device__ __forceinline__ long long pages_of(long long tokens) { return (tokens + kKvPage - 1) / kKvPage; }
 
@@ -72,9 +73,19 @@ __device__ __forceinline__ long long block_min(long long v, long long* red) {
   return v;
 }
 
+// What a row needs of the requests: in global memory, or in shared memory where
+// the CTA that made it places the rows too.
+struct PlanView {
+  const int* row_start;   // [n + 1]
+  const int* page_start;  // [n]
+  const int* held;        // [n] tokens before the step
+  const int* status;      // [n]
+  const int* parents;     // [rows]
+};
+
 // One row of the step: its request, position and slot, the page it is the
 // first on, and the mask of its node's path.
-__device__ __forceinline__ void plan_row(const PlanArgs& a, int r, int total, int top) {
+__device__ __forceinline__ void plan_row(const PlanArgs& a, const PlanView& q, int r, int total, int top) {
   int req = -1, pos = -1, slot = -1;
   bool walk = false;
   int i = 0, j = 0;
@@ -82,25 +93,25 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, int r, int total, in
     int lo = 0, hi = a.n - 1;  // the request whose rows hold r: the first with row_start[i + 1] > r
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (a.out.row_start[mid + 1] > r) hi = mid;
+      if (q.row_start[mid + 1] > r) hi = mid;
       else lo = mid + 1;
     }
     i = req = lo;
-    j = r - a.out.row_start[i];
-    if (a.out.status[i] == 0) {
-      const int len = a.out.lengths[i] - a.counts[i];
+    j = r - q.row_start[i];
+    if (q.status[i] == 0) {
+      const int len = q.held ? q.held[i] : a.out.lengths[i] - a.counts[i];
       const int p = len + j, idx = p / kKvPage, held = (int)pages_of(len);
       int* entry = a.tables + (size_t)i * a.ld_tables + idx;
       int page;
       if (idx >= held) {
-        page = a.free_pages[top - 1 - (a.out.page_start[i] + idx - held)];
+        page = a.free_pages[top - 1 - (q.page_start[i] + idx - held)];
         if (p % kKvPage == 0) *entry = page;
       } else {
         page = *entry;
       }
       pos = p;
       if (page >= 0 && page < INT_MAX / kKvPage) slot = page * kKvPage + p % kKvPage;
-      walk = a.parents != nullptr;
+      walk = q.parents != nullptr;
     }
   }
   if (a.words > 0) {
@@ -110,7 +121,7 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, int r, int total, in
     int w = a.words - 1;
     unsigned acc = 0;
     if (walk) {
-      const int* parents = a.parents + (r - j);
+      const int* parents = q.parents + (r - j);
       int node = j, depth = 0;
       while (true) {
         const int nw = node >> 5;
@@ -140,8 +151,11 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, int r, int total, in
   a.out.slots[r] = slot;
 }
 
+// with_rows: the rows too (a.n <= kPlanThreads, a.rows <= kPlanRows)
 __global__ void __launch_bounds__(kPlanThreads) k_plan(const PlanArgs a, int with_rows) {
   __shared__ long long red[kPlanWarps];
+  __shared__ int s_row[kPlanThreads + 1], s_page[kPlanThreads], s_held[kPlanThreads], s_status[kPlanThreads];
+  __shared__ int s_parents[kPlanRows];
   const int tid = threadIdx.x;
   pdl_wait();
   pdl_trigger();
@@ -170,6 +184,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const PlanArgs a, int wit
     cut = first < cut ? first : cut;
     if (in) {
       const long long row0 = row_end - ext, page0 = page_end - need;
+      if (with_rows) {
+        s_row[tid] = (int)(row0 < a.rows ? row0 : a.rows);
+        s_page[tid] = (int)(page0 < cut ? page0 : cut);
+        s_held[tid] = len;
+        s_status[tid] = status;
+      }
       a.out.row_start[i] = (int)(row0 < a.rows ? row0 : a.rows);
       a.out.page_start[i] = (int)(page0 < cut ? page0 : cut);
       a.out.status[i] = status;
@@ -185,8 +205,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const PlanArgs a, int wit
     *a.out.free_count = top - taken;
   }
   if (!with_rows) return;
+  if (tid == 0) s_row[a.n] = total;
+  if (a.parents)
+    for (int r = tid; r < a.rows; r += kPlanThreads) s_parents[r] = a.parents[r];
   __syncthreads();
-  for (int r = tid; r < a.rows; r += kPlanThreads) plan_row(a, r, total, top);
+  const PlanView q = {s_row, s_page, s_held, s_status, a.parents ? s_parents : nullptr};
+  for (int r = tid; r < a.rows; r += kPlanThreads) plan_row(a, q, r, total, top);
 }
 
 __global__ void __launch_bounds__(256) k_plan_rows(const PlanArgs a) {
@@ -195,8 +219,11 @@ __global__ void __launch_bounds__(256) k_plan_rows(const PlanArgs a) {
   const int total = a.out.row_start[a.n];
   const int top = *a.out.free_count + a.out.page_start[a.n];
   const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r < a.rows) plan_row(a, r, total, top);
+  const PlanView q = {a.out.row_start, a.out.page_start, nullptr, a.out.status, a.parents};
+  if (r < a.rows) plan_row(a, q, r, total, top);
 }
+
+constexpr int kOwnPages = 8;
 
 __global__ void __launch_bounds__(kPlanThreads) k_release(const ReleaseArgs a) {
   __shared__ long long red[kPlanWarps];
@@ -212,10 +239,18 @@ __global__ void __launch_bounds__(kPlanThreads) k_release(const ReleaseArgs a) {
     const int len = in ? a.lengths[i] : 0, keep = in ? min(a.keep[i], len) : 0;
     int status = len < 0 || keep < 0 || len > limit ? WL_STEP_BAD_REQUEST : 0;
     const int p0 = status ? 0 : (int)pages_of(keep), p1 = status ? 0 : (int)pages_of(len);
-    // a warp looks at the pages of its 32 requests together
-    for (unsigned todo = __ballot_sync(0xffffffffu, p1 > p0); todo; todo &= todo - 1) {
+    // a thread looks at its request's first pages, a warp together at the rest
+    {
+      const int* row = a.tables + (size_t)i * a.ld_tables;
+      bool hole = false;
+#pragma unroll
+      for (int q = 0; q < kOwnPages; q++)
+        if (p0 + q < p1) hole |= row[p0 + q] < 0;
+      if (hole) status = WL_STEP_TABLE_FULL;
+    }
+    for (unsigned todo = __ballot_sync(0xffffffffu, p1 > p0 + kOwnPages); todo; todo &= todo - 1) {
       const int src = __ffs(todo) - 1;
-      const int q0 = __shfl_sync(0xffffffffu, p0, src), q1 = __shfl_sync(0xffffffffu, p1, src);
+      const int q0 = __shfl_sync(0xffffffffu, p0, src) + kOwnPages, q1 = __shfl_sync(0xffffffffu, p1, src);
       const int* row = a.tables + (size_t)(i0 + warp * 32 + src) * a.ld_tables;
       bool hole = false;
       for (int q = q0 + lane; q < q1; q += 32) hole |= row[q] < 0;
@@ -374,7 +409,7 @@ int append_t(const void* k, const void* v, size_t ldk, size_t ldv, const int* sl
 // The rows join the scan's CTA while there are few of them; past that the
 // scatter takes a launch of its own over the whole GPU.
 int launch_block_tables(const PlanArgs& a, cudaStream_t st) {
-  const bool one = a.rows <= kPlanThreads * 4;
+  const bool one = a.rows <= kPlanRows && a.n <= kPlanThreads;
   WL_TRY(launch_step(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, one ? 1 : 0));
   if (!one) WL_TRY(launch_step(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a));
   return WL_OK;
