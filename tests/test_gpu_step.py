@@ -718,3 +718,29 @@ def test_a_captured_step():
         for x, y in zip(got[9:11], want[9:11]):
             assert torch.equal(x[:n], y[:n])
         assert torch.equal(got[11], want[11])
+
+
+def test_engine_rules_on_the_gpu_match_the_host(tiny_models):
+    """The batched engine with penalties, biases and a grammar gives the same
+    tokens whether the rules and the sampling run on the GPU or on the host."""
+    from woolly_b200.engine import BatchEngine, GenerationConfig
+    from woolly_b200.model import CudaTransformer
+    rng = np.random.default_rng(7)
+    prompts = [rng.integers(3, 1024, n).tolist() for n in (5, 9, 3, 12)]
+    cfgs = [GenerationConfig(max_tokens=9, eos_below=0, repetition_penalty=1.4, frequency_penalty=0.3),
+            GenerationConfig(max_tokens=9, eos_below=0, temperature=0.9, top_k=30, seed=2,
+                             logit_bias={t: float(b) for t, b in zip(range(3, 400, 7), rng.normal(0, 2, 57))}),
+            GenerationConfig(max_tokens=9, eos_below=0),
+            GenerationConfig(max_tokens=9, eos_below=0, temperature=0.7, seed=5, presence_penalty=0.5,
+                             allowed=lambda t: range(len(t), 1000, 3) if len(t) < 7 else [])]
+    runs = []
+    for dev in (False, True):
+        m = CudaTransformer(tiny_models["gqa_q4_0"], max_sessions=4, max_context=64, max_batch=4)
+        eng = BatchEngine(m, device_sampling=dev)
+        ids = [eng.submit(p, c) for p, c in zip(prompts, cfgs)]
+        eng.run()
+        runs.append([(eng.finished[i].tokens, eng.finished[i].reason) for i in ids])
+        eng.close()
+        m.close()
+    assert runs[0] == runs[1]
+    assert runs[0][3][1] == "constraint" and len(runs[0][3][0]) == 7

@@ -15,6 +15,11 @@ apply_top_p_filtering: inference.rs:551-630): temperature floor 0.01, top-k
 by the k-th largest probability, top-p by the first prefix whose cumulative
 probability exceeds p, greedy (temperature == 0) as the last index of the
 largest probability, and a stop on token ids below 3 (inference.rs:414-418).
+
+Before sampling, a request's logits may go through rules that the reference
+does not have: penalties for tokens that its prompt or output holds, biases and
+a grammar's mask of the tokens that may follow (GenerationConfig; apply_rules on
+the host, wl_process_logits on the GPU).
 """
 from __future__ import annotations
 
@@ -34,6 +39,17 @@ class GenerationConfig:
     top_p: float = 1.0         # 1: off
     eos_below: int = 3         # stop once a token id < eos_below is produced (0: never)
     seed: int = 0              # per-request sampling stream
+    repetition_penalty: float = 1.0  # logits of seen tokens: divided if positive, else multiplied (1: off)
+    presence_penalty: float = 0.0    # taken off the logits of produced tokens, once
+    frequency_penalty: float = 0.0   # and once for each time that they were produced
+    logit_bias: dict | None = None   # token id -> added to its logit
+    # callable(tokens produced so far) -> ids that may follow, a boolean mask over the
+    # vocabulary, or None for any; an empty answer ends the request ("constraint")
+    allowed: object = None
+
+    def has_rules(self) -> bool:
+        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0
+                or self.frequency_penalty != 0.0 or bool(self.logit_bias) or self.allowed is not None)
 
 
 def softmax_with_temperature(logits: np.ndarray, temperature: float) -> np.ndarray:
@@ -97,6 +113,78 @@ def sample_from_distribution(probs: np.ndarray, rng: np.random.Generator) -> int
     return int(hit[0]) if hit.size else probs.size - 1
 
 
+def allowed_mask(cfg: GenerationConfig, tokens, vocab: int) -> np.ndarray | None:
+    """Boolean mask of the ids that may follow `tokens`, or None when any may."""
+    if cfg.allowed is None:
+        return None
+    ids = cfg.allowed(list(tokens))
+    if ids is None:
+        return None
+    ids = np.asarray(ids if isinstance(ids, np.ndarray) else list(ids))
+    if ids.dtype == np.bool_:
+        if ids.shape != (vocab,):
+            raise ValueError(f"allowed() must give {vocab} truth values, got {ids.shape}")
+        return ids
+    m = np.zeros(vocab, bool)
+    if ids.size:
+        if ids.min() < 0 or ids.max() >= vocab:
+            raise ValueError("allowed() gave an id outside the vocabulary")
+        m[ids.astype(np.int64)] = True
+    return m
+
+
+def apply_rules(logits: np.ndarray, cfg: GenerationConfig, prompt, tokens,
+                mask: np.ndarray | None = None) -> np.ndarray:
+    """wl_process_logits' rules on one row, in f32: penalties for the tokens of
+    the prompt (repetition) and of the output, biases, then the mask."""
+    x = np.array(logits, np.float32, copy=True)
+    V = x.size
+    made = np.bincount(np.asarray([t for t in tokens if 0 <= t < V], np.int64), minlength=V)
+    seen = made > 0
+    seen[np.asarray([t for t in prompt if 0 <= t < V], np.int64)] = True
+    r = np.float32(cfg.repetition_penalty)
+    x[seen] = np.where(x[seen] > 0, x[seen] / r, x[seen] * r)
+    hit = made > 0
+    x[hit] -= np.float32(cfg.frequency_penalty) * made[hit].astype(np.float32) + np.float32(cfg.presence_penalty)
+    for t, b in (cfg.logit_bias or {}).items():
+        x[t] += np.float32(b)
+    if mask is not None:
+        x[~mask] = -np.inf
+    return x
+
+
+def pack_rules(requests, masks, vocab: int) -> dict:
+    """The rules of a batch's rows (requests with cfg, prompt and tokens; their
+    masks or None) as host arrays, keyed as process_logits and logit_params
+    take them."""
+    def starts(lists):
+        return np.concatenate([[0], np.cumsum([len(x) for x in lists])]).astype(np.int32)
+
+    def flat(lists, dtype):
+        return np.concatenate([np.asarray(x, dtype) for x in lists]) if lists else np.zeros(0, dtype)
+    hist = [r.prompt + r.tokens for r in requests]
+    bias = [list((r.cfg.logit_bias or {}).items()) for r in requests]
+    row, words = np.full(len(requests), -1, np.int32), []
+    for i, m in enumerate(masks):
+        if m is not None:
+            row[i] = len(words)
+            bits = np.zeros(-(-vocab // 32) * 32, np.uint8)
+            bits[:vocab] = m
+            words.append(np.packbits(bits, bitorder="little").view(np.uint32).view(np.int32))
+    out = dict(
+        params=dict(repetition=[r.cfg.repetition_penalty for r in requests],
+                    presence=[r.cfg.presence_penalty for r in requests],
+                    frequency=[r.cfg.frequency_penalty for r in requests], allowed_row=row),
+        history=flat(hist, np.int32), history_start=starts(hist),
+        prompt_lens=np.asarray([len(r.prompt) for r in requests], np.int32))
+    if any(bias):
+        out.update(bias_start=starts(bias), bias_tokens=flat([[t for t, _ in b] for b in bias], np.int32),
+                   bias_values=flat([[v for _, v in b] for b in bias], np.float32))
+    if words:
+        out["allowed"] = np.stack(words)
+    return out
+
+
 @dataclass
 class Request:
     rid: int
@@ -120,7 +208,7 @@ class BatchEngine:
     token), then decodes one token for every other running request in one
     batched forward; run() steps until every request has finished.  A request
     finishes after cfg.max_tokens tokens, on a token id below cfg.eos_below,
-    or when its session's context is full.  Its session is released at once,
+    when its session's context is full, or when its grammar allows nothing.  Its session is released at once,
     so a waiting request can take the slot on the next step.
     """
 
@@ -152,14 +240,34 @@ class BatchEngine:
         if not prompt:
             raise ValueError("empty prompt (the reference's EMPTY_INPUT)")
         cfg = cfg or GenerationConfig()
+        if not (np.isfinite(cfg.repetition_penalty) and cfg.repetition_penalty > 0):
+            raise ValueError("repetition_penalty must be positive and finite")
+        if not (np.isfinite(cfg.presence_penalty) and np.isfinite(cfg.frequency_penalty)):
+            raise ValueError("presence_penalty and frequency_penalty must be finite")
+        for t, b in (cfg.logit_bias or {}).items():
+            if not (0 <= t < self.model.vocab_size()) or np.isnan(b):
+                raise ValueError(f"logit_bias: token {t} outside the vocabulary, or not a number")
         r = Request(self._next, prompt, cfg, np.random.default_rng(cfg.seed), on_token=on_token)
         self._next += 1
         self.waiting.append(r)
         return r.rid
 
     # ---------------------------------------------------------------- internals
+    def _mask(self, r: Request) -> np.ndarray | None:
+        """The request's mask; one that leaves nothing ends the request."""
+        m = allowed_mask(r.cfg, r.tokens, self.model.vocab_size())
+        if m is not None and not m.any():
+            r.done, r.reason = True, "constraint"
+        return m
+
     def _emit(self, r: Request, row: np.ndarray) -> None:
-        tok = sample_next_token(row, r.cfg, r.rng)
+        ruled = row
+        if r.cfg.has_rules():
+            mask = self._mask(r)
+            if r.done:
+                return
+            ruled = apply_rules(row, r.cfg, r.prompt, r.tokens, mask)
+        tok = sample_next_token(ruled, r.cfg, r.rng)
         if self.keep_logits:
             r.logits.append(np.array(row, np.float32, copy=True))
         self._emit_token(r, tok)
@@ -214,7 +322,14 @@ class BatchEngine:
         for r in new:  # prefill: the prompt's last row gives the first token
             row = self.model.forward_sessions([r.session], [r.prompt])[0]
             self._emit(r, np.asarray(row).reshape(-1)[-self.model.vocab_size():])
-            produced += 1
+            produced += len(r.tokens)
+        if decoding and self.device_sampling:
+            kw = {}
+            if any(r.cfg.has_rules() for r in decoding):
+                masks = [self._mask(r) for r in decoding]
+                masks = [m for m, r in zip(masks, decoding) if not r.done]
+                decoding = [r for r in decoding if not r.done]
+                kw["rules"] = pack_rules(decoding, masks, self.model.vocab_size())
         if decoding and self.device_sampling:
             cf = [r.cfg for r in decoding]
             u = [np.float32(r.rng.random(dtype=np.float32)) if r.cfg.temperature != 0.0 else 0.0
@@ -222,7 +337,7 @@ class BatchEngine:
             toks = self.model.decode_sample([r.session for r in decoding],
                                             [r.tokens[-1] for r in decoding],
                                             [c.temperature for c in cf], [c.top_k for c in cf],
-                                            [c.top_p for c in cf], u)
+                                            [c.top_p for c in cf], u, **kw)
             for r, tok in zip(decoding, toks):
                 self._emit_token(r, tok)
                 produced += 1
@@ -230,8 +345,9 @@ class BatchEngine:
             outs = self.model.forward_sessions([r.session for r in decoding],
                                                [[r.tokens[-1]] for r in decoding])
             for r, row in zip(decoding, outs):
+                n = len(r.tokens)
                 self._emit(r, np.asarray(row).reshape(-1))
-                produced += 1
+                produced += len(r.tokens) - n
         self.running += new
         self._retire()
         return produced

@@ -175,13 +175,15 @@ class CudaTransformer:
 
 
     def decode_sample(self, sessions: Sequence["Session"], ids: Sequence[int], temperature=0.0,
-                      top_k=0, top_p=1.0, u=0.0) -> np.ndarray:
+                      top_k=0, top_p=1.0, u=0.0, rules: dict | None = None) -> np.ndarray:
         """One batched decode step that returns the next token of every
         session, sampled on the GPU by the server's rules (wl_sample;
         inference.rs:441-483): the step's ids go to the device, only the
         sampled ids come back (4 bytes per session instead of a row of
         logits).  temperature / top_k / top_p / u are scalars or per-session
-        sequences; u is the uniform draw of each session's sampling stream."""
+        sequences; u is the uniform draw of each session's sampling stream.
+        rules (engine.pack_rules): penalties, biases and masks that the logits
+        go through before sampling (wl_process_logits)."""
         import torch
         from . import ops
         n = len(sessions)
@@ -201,10 +203,28 @@ class CudaTransformer:
         stream = torch.cuda.current_stream(dev)
         d_ids[:n].copy_(h_ids[:n], non_blocking=True)
         self.decode_step_device(sessions, d_ids.data_ptr(), d_logits.data_ptr(), stream.cuda_stream)
+        if rules is not None:
+            self._apply_rules(d_logits[:n], rules, dev)
         ops.sample(d_logits[:n], temperature, top_k, top_p, u, out=d_next[:n], params=d_prm)
         h_next[:n].copy_(d_next[:n], non_blocking=True)
         stream.synchronize()
         return h_next[:n].numpy().copy()
+
+    @staticmethod
+    def _apply_rules(logits, rules: dict, dev) -> None:
+        """process_logits in place on rows of logits; the rules' arrays cross in one copy."""
+        import torch
+        from . import ops
+        rules = dict(rules)
+        prm = ops.logit_params(logits.shape[0], device="cpu", **rules.pop("params"))
+        arrays = {"params": prm.numpy().view(np.int32), **rules}
+        flat = np.concatenate([a.reshape(-1).view(np.int32) for a in arrays.values()])
+        buf, at, kw = torch.from_numpy(flat).to(dev), 0, {}
+        for name, a in arrays.items():
+            t = buf[at:at + a.size].view(a.shape)
+            kw[name] = t.view(torch.float32) if a.dtype == np.float32 else t
+            at += a.size
+        ops.process_logits(logits, kw.pop("params").view(torch.uint8), out=logits, **kw)
 
 
 class Session:
