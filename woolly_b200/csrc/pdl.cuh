@@ -12,6 +12,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <utility>
 
 #include "common.h"
@@ -49,10 +50,12 @@ int launch_k(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStr
 // launch_k with the attribute set whatever the thread's setting: for the
 // operators of a serving step, whose kernels all wait (pdl_wait) before they
 // touch global memory.  A launch then costs its set-up under the kernel before it.
+// WL_NO_PDL in the environment turns it off here too.
 template <class... KArgs, class... Args>
 int launch_step(void (*kern)(KArgs...), Args&&... args) {
+  static const bool on = getenv("WL_NO_PDL") == nullptr;
   const bool was = pdl_enabled();
-  set_pdl(true);
+  set_pdl(on);
   const int s = launch_k(kern, std::forward<Args>(args)...);
   set_pdl(was);
   return s;
