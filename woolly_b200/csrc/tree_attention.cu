@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         const int b = buf(u), t = NS == 2 ? u & 1 : 0;
         const uint32_t k = seq + v_at(pair ? u >> 1 : u), slot = k % NSLOT, parity = np >> b & 1;
         np ^= 1u << b;
-        if (!wait(pbar + 8 * b, parity) || !wait(full + 8 * slot, (k / NSLOT) & 1)) break;
+        if (!wait(full + 8 * slot, (k / NSLOT) & 1) || !wait(pbar + 8 * b, parity)) break;
         fence_after();
         const uint32_t vb = desc_lo(ring + slot * S::kSlot, KT * 128);
         const uint32_t d = tm + S::kO + t * HD, p = tm + b * KT;
@@ -827,22 +827,18 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           // the scores, 32 at a time: for the maximum, and again for P (held in
           // between, 64 of them push the loop's state out of registers)
           const bool masked = key0 < open0 || key0 + KT > len;
-          uint32_t see[CW / 32];
-          if (masked) {
-#pragma unroll
-            for (int k = 0; k < CW / 32; k++) see[k] = visible(key0 + hf * CW + 32 * k);
-            __syncwarp();
-          }
           float s[32], top = -INFINITY;
           auto load = [&](int k) {
             tm_ld32(sp + k * 32, reinterpret_cast<uint32_t*>(s));
             tm_wait_ld(reinterpret_cast<uint32_t*>(s));
             if (masked) {
+              const uint32_t see = visible(key0 + hf * CW + 32 * k);
 #pragma unroll
-              for (int e = 0; e < 32; e++) s[e] = see[k] >> e & 1u ? s[e] : -INFINITY;
+              for (int e = 0; e < 32; e++) s[e] = see >> e & 1u ? s[e] : -INFINITY;
+              __syncwarp();
             }
           };
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < CW / 32; k++) {
             load(k);
             float t4[4] = {s[0], s[1], s[2], s[3]};
@@ -880,7 +876,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
           const f2 c2 = make_f2(c, c), off2 = make_f2(off, off);
           f2 sum[2] = {make_f2(0.f, 0.f), make_f2(0.f, 0.f)};
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < CW / 32; k++) {
             if (CW > 32) load(k);
             // over the scores they came from: 16 columns of high words, then low ones
@@ -1046,9 +1042,6 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
   pdl_trigger();
   if (head >= a.heads || r >= min(a.row_start[a.n], a.rows)) return;
   const long long per = parts.start[a.n + 1];
-  bool failed = false;
-  for (int c = lane; c < ctas; c += 32) failed |= parts.status[c] != 0;
-  failed = __any_sync(0xffffffffu, failed);
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -1064,6 +1057,7 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
   const int c0 = (int)quot(g0, per), c1 = (int)quot(g1 - 1, per);
   // parts: both streams of each CTA of the group, or the query tile's own
   const int nt = w == 2 ? 1 : S::NS, np = (c1 - c0 + 1) * nt;
+  bool failed = false;
   float M = -INFINITY, L = 0.f, o[HD / 32];
 #pragma unroll
   for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
@@ -1072,6 +1066,7 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
     const long long s = max((long long)c * per, g0), e1 = min((long long)(c + 1) * per, g1);
     const int ta = (int)((s - g0) >> (w - 1)), tb = (int)((e1 - g0) >> (w - 1));
     const bool ok = p < np && tb > ta && (w == 2 || t < tb - ta);
+    failed |= __any_sync(0xffffffffu, p < np && parts.status[min(c, ctas - 1)] != 0);
     if (__any_sync(0xffffffffu, ok && ta == 0 && tb == q.kt)) {  // one CTA had it all and wrote the row
       if (!failed) return;
       break;
