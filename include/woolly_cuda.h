@@ -388,7 +388,8 @@ int wl_kv_commit(int cache_type, const int* tables, int ld_tables, int max_pages
  * wl_block_tables' slots; `lengths` are those given to it).  A row attends the
  * cached tokens and the step's own tokens named by its mask bits (its own
  * among them); without a mask the earlier tokens of its request and itself.
- * window > 0 keeps keys at positions > positions[r] - window.  Rows with a
+ * window > 0 keeps keys at positions > positions[r] - window (the rows' positions
+ * are lengths[i] or more; smaller ones count as lengths[i]).  Rows with a
  * negative position, and rows with nothing to attend, give zeros; rows behind
  * row_start[n] are left as they were.  Keys on pages outside the cache are
  * masked.  q and out are f32 over an f16 cache, or f16 / bf16 over a cache of
@@ -428,8 +429,8 @@ typedef struct wl_logit_context {
   const uint32_t* draft_mask; /* [rows][words] */
   int words;
   const int* row_start;       /* [n_history + 1] */
-  /* biases of row r: entries bias_start[r] .. bias_start[r + 1); of several
-   * for one token the last holds; bias_total is their number */
+  /* biases of row r: entries bias_start[r] .. bias_start[r + 1) (starts do not
+   * fall); of several for one token the last holds; bias_total is their number */
   const int *bias_start, *bias_tokens;
   const float* bias_values;
   int bias_total;

@@ -217,6 +217,23 @@ def test_release_parts_in_place():
     assert (t[0] == -1).all() and t[1].tolist() == [5, 6, -1, 8, 9] and t[7].tolist() == T[7].tolist()
 
 
+@pytest.mark.parametrize("n,rows", [(40, 200), (40, 9000), (1300, 1500)])
+def test_block_tables_in_place(n, rows):
+    """The new lengths and the free count on the arguments themselves, step after step."""
+    rng = np.random.default_rng(rows)
+    _, _, T, free = make_step(rng, n, 0, 1, 60 * n, pages=40)
+    t, f, L, c = i32(T), i32(free), i32(np.zeros(n)), i32([len(free)])
+    lengths, top = np.zeros(n, np.int64), len(free)
+    out = ops.step_plan(n, rows)._replace(lengths=L, free_count=c)
+    for _ in range(4):
+        counts = rng.integers(0, 30 if rows > 5000 else 4, n)
+        want, T = ref_plan(T, lengths, counts, free, top, rows)
+        ops.block_tables(t, L, i32(counts), f, c, rows, out=out)
+        check_plan(out, want, 0)
+        assert np.array_equal(t.cpu().numpy(), T)
+        lengths, top = np.array(want["lengths"]), want["free_count"][0]
+
+
 # ------------------------------------------------------------------ cache writes
 @pytest.mark.parametrize("src,cache", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
 @pytest.mark.parametrize("rows,kvh,hd", [(1, 1, 8), (5, 3, 64), (70, 8, 128), (33, 2, 256), (300, 5, 40)])
@@ -496,6 +513,63 @@ def test_attention_repeats_exactly():
     first = call_attention(a)
     for _ in range(3):
         assert torch.equal(first, call_attention(a))
+
+
+@pytest.mark.parametrize("qt", [F32, BF16])
+def test_attention_many_requests(qt):
+    """More requests than a CTA has threads."""
+    rng = np.random.default_rng(1)
+    a = make_attention(12, rng.integers(0, 40, 1500), rng.integers(0, 3, 1500), 2, 1, 64, qt)
+    close(call_attention(a), *ref_attention(a))
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+def test_attention_small_positions_and_narrow_masks(hd):
+    """Positions below the context's length count as it; nodes past the mask's
+    width are seen by nobody."""
+    a = make_attention(13, [70, 20], [40, 50], 2, 1, hd, F16)
+    pos = a["pos"].copy()
+    a["pos"] = np.where(np.arange(90) % 3 == 0, 5, pos)
+    low = dict(a, pos=np.maximum(a["pos"], np.repeat([70, 20], [40, 50])))
+    close(call_attention(a, 30), *ref_attention(low, 30))
+    narrow = dict(a, pos=pos, mask=np.ascontiguousarray(a["mask"][:, :1]))
+    close(call_attention(narrow), *ref_attention(narrow))
+
+
+def test_attention_on_two_streams_at_once():
+    a, b = (make_attention(s, [900, 40], [20, 3], 8, 2, 128, BF16) for s in (14, 15))
+    wa, wb = ref_attention(a), ref_attention(b)
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(6):
+        with torch.cuda.stream(sa):
+            got.append((call_attention(a), wa))
+        with torch.cuda.stream(sb):
+            got.append((call_attention(b), wb))
+    torch.cuda.synchronize()
+    for g, w in got:
+        close(g, *w)
+
+
+def test_a_cache_past_32_bit_offsets():
+    """Pages whose elements lie beyond 2^32 bytes and 2^31 elements."""
+    kvh, hd, pages = 8, 128, 139000  # 2.28e9 elements per cache
+    if torch.cuda.mem_get_info()[0] < 30e9:
+        pytest.skip("needs 10 GB")
+    a = make_attention(16, [100, 33], [3, 20], 16, kvh, hd, F16)
+    used = a["ck"].shape[0]
+    big = [torch.empty(pages, kvh, P, hd, dtype=F16, device="cuda") for _ in range(2)]
+    for x, small in zip(big, (a["ck"], a["cv"])):
+        x[pages - used:] = small
+    far = dict(a, ck=big[0], cv=big[1], tables=np.where(a["tables"] >= 0, a["tables"] + pages - used, -1))
+    assert torch.equal(call_attention(far), call_attention(a))
+    k, v = (torch.randn(2, kvh, hd, device="cuda") for _ in range(2))
+    slots = i32([pages * P - 1, (pages - 1) * P])
+    ops.kv_append(k, v, slots, *big)
+    assert torch.equal(big[0][-1, :, 15], k[0].to(F16)) and torch.equal(big[1][-1, :, 0], v[1].to(F16))
+    ops.kv_commit(i32([[pages - 1]]), i32([0]), i32([15]), i32([0, 1]), *big)
+    assert torch.equal(big[0][-1, :, 0], k[0].to(F16))
 
 
 # ------------------------------------------------------------------ logits

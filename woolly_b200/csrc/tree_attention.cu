@@ -66,15 +66,16 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
   const int r = blockIdx.x, head = blockIdx.y, hd = a.head_dim, kvh = head / (a.heads / a.kv_heads);
   pdl_wait();
   pdl_trigger();
-  if (r >= a.row_start[a.n]) return;
+  if (r >= min(a.row_start[a.n], a.rows)) return;
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (a.row_start[mid + 1] > r) hi = mid;
     else lo = mid + 1;
   }
-  const int i = lo, row0 = a.row_start[i], T = a.row_start[i + 1] - row0;
-  const int pos = a.pos[r], len = max(a.lengths[i], 0);
+  const int i = lo, row0 = max(a.row_start[i], 0), T = min(a.row_start[i + 1], a.rows) - row0;
+  const int len = (int)min((long long)max(a.lengths[i], 0), (long long)a.max_pages * kKvPage);
+  const int pos = a.pos[r] < 0 ? -1 : max(a.pos[r], len);
   const Q* q = (const Q*)a.q + (size_t)r * a.ldq + (size_t)head * hd;
   for (int d = tid; d < hd; d += 128) s_q[d] = as_f32(q[d]);
   __syncthreads();
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
       if (t >= len) {
         const int c = t - len;
         ok = a.mask ? c < 32 * a.words && (a.mask[(size_t)r * a.words + (c >> 5)] >> (c & 31) & 1u) : c <= r - row0;
-        at = a.pos[row0 + c];
+        at = max(a.pos[row0 + c], len);
       }
       if (a.window > 0) ok = ok && at > pos - a.window;
       const int page = ok ? a.tables[(size_t)i * a.ld_tables + t / kKvPage] : -1;
@@ -797,7 +798,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           if (a.window > 0)
             for (uint32_t left = own; left; left &= left - 1) {
               const int bit = __ffs(left) - 1;
-              if (a.pos[run.row0 + c0 + bit] <= pos - a.window) own &= ~(1u << bit);
+              if (max(a.pos[run.row0 + c0 + bit], len) <= pos - a.window) own &= ~(1u << bit);
             }
           see |= own;
         }

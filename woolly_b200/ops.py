@@ -477,7 +477,7 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     tokens and the tokens of the step that its mask bits name (block_tables'
     mask); without a mask, the step's earlier tokens and itself, so that one
     row per request is a plain decode step.  `window` > 0 keeps keys at
-    positions > positions[r] - window (positions count from lengths[i] on);
+    positions > positions[r] - window (positions below lengths[i] count as it);
     `scale` defaults to head_dim ** -0.5.
     A row with a negative position or nothing to attend gives zeros; rows
     behind row_start[n] are not written.  q is f32 over an f16 cache, or has
