@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         return row;
       };
-      int before = rows_end, now = fetch(0), after = fetch(1), at = 0;
+      int before = rows_end, now = fetch(0), after = nt > 32 / PAGES ? fetch(1) : rows_end, at = 0;
       auto load = [&](const CUtensorMap* map, int tile) {
         if (!ok) return;
         const int batch = tile / (32 / PAGES);

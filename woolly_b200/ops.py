@@ -325,10 +325,9 @@ class Released(NamedTuple):
 
 def step_plan(n: int, rows: int, words: int = 0, device="cuda") -> StepPlan:
     """Buffers for block_tables' `out`: n requests, `rows` rows, masks of `words` words."""
-    # one allocation; the row arrays come first
-    b = torch.empty(3 * rows + 4 * n + 3, dtype=_I32, device=device)
-    req, pos, slot, lengths, status, start, pages, free = b.split_with_sizes(
-        (rows, rows, rows, n, n, n + 1, n + 1, 1))
+    b = torch.empty(3 * rows + 4 * n + 3, dtype=_I32, device=device)  # one allocation, cut up
+    req, pos, slot, lengths, status, start, pages, free = torch.unsafe_split_with_sizes(
+        b, (rows, rows, rows, n, n, n + 1, n + 1, 1))
     return StepPlan(start, req, pos, slot, lengths, status, free, pages,
                     torch.empty((rows, words), dtype=_I32, device=device) if words else None)
 
@@ -368,13 +367,18 @@ def block_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tens
     par = None if parents is None else _i32(parents, "parents", (rows,), index)
     if out is None:
         out = step_plan(n, rows, words, tables.device)
+        at0 = out.requests.data_ptr() if rows else out.lengths.data_ptr() if n else out.row_start.data_ptr()
+        row0, row1, row2, len0 = at0, at0 + 4 * rows, at0 + 8 * rows, at0 + 12 * rows
+        ptrs = (len0 + 8 * n, row0, row1, row2, len0, len0 + 4 * n, len0 + 16 * n + 8, len0 + 12 * n + 4,
+                out.mask.data_ptr() if words else None)
     else:
         shapes = ((n + 1,), (rows,), (rows,), (rows,), each, each, one, (n + 1,))
         for f, t, shape in zip(StepPlan._fields, out, shapes):
             _i32(t, f"out.{f}", shape, index)
         if words:
             _i32(out.mask, "out.mask", (rows, words), index)
-    o = _lib.StepPlan(*[t if t is None else t.data_ptr() for t in out])
+        ptrs = [t if t is None else t.data_ptr() for t in out]
+    o = _lib.StepPlan(*ptrs)
     _launch(lib().wl_block_tables, index, at, ld, pages, _i32(lengths, "lengths", each, index),
             _i32(counts, "counts", each, index), n, _list32(free_pages, "free_pages", index),
             free_pages.numel(), _i32(free_count, "free_count", one, index), rows, par, words, C.byref(o))
@@ -392,7 +396,7 @@ def release_pages(tables: torch.Tensor, lengths: torch.Tensor, keep: torch.Tenso
     each, one = (n,), (1,)
     if out is None:
         b = torch.empty(3 * n + 2, dtype=_I32, device=tables.device)
-        out = Released(*b.split_with_sizes((n, n, 1, n + 1)))
+        out = Released(*torch.unsafe_split_with_sizes(b, (n, n, 1, n + 1)))
     else:
         for f, t, shape in zip(Released._fields, out, (each, each, one, (n + 1,))):
             _i32(t, f"out.{f}", shape, index)
@@ -560,46 +564,47 @@ def process_logits(logits: torch.Tensor, params: torch.Tensor, *, history: torch
         _refuse(params, "params", (torch.uint8,), (None,), index)
     if params.numel() < rows * 16:
         raise ValueError(f"params must hold {rows} records")
-    c = _lib.LogitContext()
     n, every = 0, (rows,)
+    h = h0 = hp = req = dt = dm = d0 = bs = bt = bv = al = None
+    total = words = nb = na = aw = 0
     if history_start is not None or history is not None:
-        c.history_start = _list32(history_start, "history_start", index)
-        c.history = _list32(history, "history", index)
-        c.history_total = history.numel()
+        h0 = _list32(history_start, "history_start", index)
+        h = _list32(history, "history", index)
+        total = history.numel()
         n = history_start.numel() - 1
         if n < 0:
             raise ValueError("history_start must have one entry more than there are requests")
     if prompt_lens is not None:
         if history is None:
             raise ValueError("prompt_lens needs a history")
-        c.prompt_lens = _i32(prompt_lens, "prompt_lens", (n,), index)
+        hp = _i32(prompt_lens, "prompt_lens", (n,), index)
     if draft_mask is not None or draft_tokens is not None:
         if draft_mask is None or draft_tokens is None or row_start is None:
             raise ValueError("drafts need draft_tokens, draft_mask and row_start")
-        c.words = draft_mask.shape[1] if draft_mask.dim() == 2 else 0
-        c.draft_mask = _i32(draft_mask, "draft_mask", (rows, c.words), index)
-        c.draft_tokens = _i32(draft_tokens, "draft_tokens", every, index)
-        c.row_start = _list32(row_start, "row_start", index)
+        words = draft_mask.shape[1] if draft_mask.dim() == 2 else 0
+        dm = _i32(draft_mask, "draft_mask", (rows, words), index)
+        dt = _i32(draft_tokens, "draft_tokens", every, index)
+        d0 = _list32(row_start, "row_start", index)
         if history is not None and row_start.numel() != n + 1:
             raise ValueError(f"row_start must have {n + 1} entries, got {row_start.numel()}")
         n = row_start.numel() - 1
-    c.n_history = n
     if requests is not None:
-        c.requests = _i32(requests, "requests", every, index)
+        req = _i32(requests, "requests", every, index)
     if bias_start is not None or bias_tokens is not None or bias_values is not None:
-        c.bias_start = _i32(bias_start, "bias_start", (rows + 1,), index)
-        c.bias_tokens = _list32(bias_tokens, "bias_tokens", index)
-        c.bias_total = nb = bias_tokens.numel()
+        bs = _i32(bias_start, "bias_start", (rows + 1,), index)
+        bt = _list32(bias_tokens, "bias_tokens", index)
+        nb = bias_tokens.numel()
         if (bias_values is None or bias_values.dtype is not torch.float32 or bias_values.shape != (nb,)
                 or bias_values.get_device() != index or not bias_values.is_contiguous()):
             _refuse(bias_values, "bias_values", (torch.float32,), (nb,), index)
-        c.bias_values = bias_values.data_ptr()
+        bv = bias_values.data_ptr()
     if allowed is not None:
         try:
-            c.n_allowed, c.allowed_words = allowed.shape
+            na, aw = allowed.shape
         except (AttributeError, ValueError):
             _refuse(allowed, "allowed", (_I32,), (None, None), index)
-        c.allowed = _i32(allowed, "allowed", (c.n_allowed, c.allowed_words), index)
+        al = _i32(allowed, "allowed", (na, aw), index)
+    c = _lib.LogitContext(h, h0, hp, n, total, req, dt, dm, words, d0, bs, bt, bv, nb, al, na, aw)
     if out is None:
         out = torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
     elif out.dtype is not logits.dtype or out.shape != (rows, V) or out.get_device() != index:
