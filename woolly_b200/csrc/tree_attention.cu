@@ -315,8 +315,34 @@ __device__ __forceinline__ Req request(const TreeAttnArgs& a, int i) {
   q.qt = (int)(((long long)q.T * (a.heads / a.kv_heads) + 127) / 128);
   return q;
 }
-__device__ __forceinline__ long long units(const TreeAttnArgs& a, const Req& q) {
-  return (long long)a.kv_heads * q.qt * q.kt;
+__device__ __forceinline__ long long quot(long long a, long long b) {  // a >= 0, b > 0
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
+// How the work is cut: CTA c takes units [c * per, (c + 1) * per), a unit being a
+// key tile times a query tile.  whole: every group starts at such a border (its
+// units are rounded up to a multiple of per), so that no CTA has two.
+struct Cut {
+  long long per;
+  bool whole;
+  __device__ long long pad(long long u) const { return whole ? quot(u + per - 1, per) * per : u; }
+};
+// Groups of a request and KV head: pairs of query tiles, then single ones.
+template <int NS>
+struct Groups {
+  int pairs, singles;
+  long long pair, single, all;  // units of one, and of them together
+  __device__ Groups(const Req& q, const Cut& cut) {
+    pairs = NS == 2 ? q.qt / 2 : 0;
+    singles = NS == 2 ? q.qt & 1 : q.qt;
+    pair = cut.pad(2LL * q.kt);
+    single = cut.pad(q.kt);
+    all = pairs * pair + singles * single;
+  }
+};
+template <int NS>
+__device__ __forceinline__ long long units(const TreeAttnArgs& a, const Req& q, const Cut& cut) {
+  return a.kv_heads * Groups<NS>(q, cut).all;
 }
 
 // Mask bits of nodes c0 .. c0 + 31 of a row (c0 > -32; nodes below 0: clear).
@@ -326,10 +352,6 @@ __device__ __forceinline__ uint32_t mask_bits(const TreeAttnArgs& a, int row, in
   const int w = c0 >> 5;
   const uint32_t w0 = w < a.words ? m[w] : 0u, w1 = w + 1 < a.words ? m[w + 1] : 0u;
   return __funnelshift_r(w0, w1, c0 & 31);
-}
-
-__device__ __forceinline__ long long quot(long long a, long long b) {  // a >= 0, b > 0
-  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 
 // A run of key tiles of one group: KV head kvh, query tiles qt0 .. qt0 + w - 1.
@@ -346,30 +368,33 @@ struct Run {
 };
 // Runs in flight: the TMA warp is ahead by no more than the ring's tiles, two
 // or more to a run, the others by one run.
-constexpr int kRuns = 10;
+constexpr int kRuns = 8;
 
 // Walks the CTA's share [x, x1) of the laid-out key tiles; all threads alike.
 template <int HD, class Q>
 struct Walk {
   using S = Shape<HD, Q>;
   long long x0, x, x1, base;  // base: start of request i
+  Cut cut;
   int i;
   Req q;
   __device__ bool next(const TreeAttnArgs& args, Run& r) {
     while (x < x1) {
-      while (x >= base + units(args, q)) {
-        base += units(args, q);
-        q = request<S::KT>(args, ++i);
-      }
-      const long long per = (long long)q.qt * q.kt;
+      for (long long u; x >= base + (u = units<S::NS>(args, q, cut)); q = request<S::KT>(args, ++i)) base += u;
+      const Groups<S::NS> g(q, cut);
       const long long off = x - base;
-      r.kvh = (int)quot(off, per);
-      const long long y = off - r.kvh * per;
-      r.qt0 = (int)quot(y, (long long)S::NS * q.kt) * S::NS;
-      r.w = min(S::NS, q.qt - r.qt0);
-      const long long g0 = base + r.kvh * per + (long long)r.qt0 * q.kt;
-      const long long g1 = g0 + (long long)r.w * q.kt, e = min(x1, g1);
-      const int ta = (int)((x - g0) >> (r.w - 1)), tb = (int)((e - g0) >> (r.w - 1));  // w is 1 or 2
+      r.kvh = (int)quot(off, g.all);
+      long long y = off - r.kvh * g.all, size = g.pair, g0 = base + r.kvh * g.all;
+      const long long paired = g.pairs * g.pair;
+      r.w = y < paired ? 2 : 1;
+      r.qt0 = 0;
+      if (r.w == 1) y -= paired, g0 += paired, r.qt0 = 2 * g.pairs, size = g.single;
+      const int idx = (int)quot(y, size);
+      r.qt0 += idx * r.w;
+      g0 += idx * size;
+      const long long e = min(x1, g0 + size);
+      const int ta = (int)min((long long)q.kt, (x - g0) >> (r.w - 1));  // w is 1 or 2
+      const int tb = (int)min((long long)q.kt, (e - g0) >> (r.w - 1));
       r.nt = tb - ta;
       r.key0 = (q.tile0 + ta) * S::KT;
       r.len = q.len, r.keys = q.keys, r.row0 = q.row0, r.T = q.T, r.i = i;
@@ -386,7 +411,7 @@ struct Walk {
 // each; one status word per CTA and the requests' prefix sums before them.
 struct Parts {
   int* status;       // [ctas]
-  long long* start;  // [n] prefix sums, then the total and a CTA's share
+  long long* start;  // [n] prefix sums, then the total and a CTA's share (negative: whole groups)
   float* o;
   float* ml;
   int prow;          // rows kept of a 128-row tile
@@ -423,7 +448,7 @@ struct Small {  // behind the tiles in shared memory
   };
   long long base;
   Req q;
-  int req, fail;
+  int req, fail, need[8];
   uint32_t tmem;
 };
 
@@ -473,6 +498,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 
   // this CTA's share of the key tiles: the total, then the request it starts in
   long long share0, share1;
+  Cut cut;
   {
     auto block_sum = [&](long long v, long long& before) {  // the sum, and that of the threads before this one
       long long x = v;
@@ -484,31 +510,64 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       __syncthreads();
       if (lane == 31) sh.scan[warp] = x;
       __syncthreads();
-      long long w = 0, all = 0;
-      for (int k = 0; k < kTaThreads / 32; k++) {
-        if (k == warp) w = all;
-        all += sh.scan[k];
+      long long w = lane < kTaThreads / 32 ? sh.scan[lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
       }
-      before = w + x - v;
-      return all;
+      const long long upto = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+      before = (warp ? upto : 0) + x - v;
+      return __shfl_sync(0xffffffffu, w, 31);
     };
     long long total = 0, before, u = 0;
     Req q{};
+    cut = Cut{1, false};
     for (int i0 = 0; i0 < a.n; i0 += kTaThreads) {
       if (i0 + tid < a.n) q = request<KT>(a, i0 + tid);
-      u = i0 + tid < a.n ? units(a, q) : 0;
+      u = i0 + tid < a.n ? units<NS>(a, q, cut) : 0;
       total += block_sum(u, before);
     }
-    const long long per = total > 0 ? quot(total + gridDim.x - 1, gridDim.x) : 1;
-    share0 = min(total, per * blockIdx.x);
-    share1 = min(total, share0 + per);
+    cut.per = total > 0 ? quot(total + gridDim.x - 1, gridDim.x) : 1;
+    // A CTA that gets the end of one group and the start of the next pays a run's
+    // fixed latency twice (about 6 us, as much as six units).  If there is a share
+    // up to seven units larger with which every group has CTAs of its own, it is
+    // taken: 5 drafted tokens over 640 keys, 32 KV heads: 21 -> 16 us.
+    if (a.n <= kTaThreads && cut.per < 4096) {
+      // a warp per candidate, over the requests' groups (in the query tiles' place)
+      int4* req = reinterpret_cast<int4*>(sm);
+      const Groups<NS> g(q, cut);
+      if (tid < a.n) req[tid] = u > 0 ? make_int4(g.pairs, g.singles, (int)g.pair, (int)g.single) : make_int4(0, 0, 0, 0);
+      __syncthreads();
+      if (warp < 8) {
+        const unsigned p = (unsigned)cut.per + warp;
+        long long ctas = 0;
+        for (int i = lane; i < a.n; i += 32) {
+          const int4 v = req[i];
+          ctas += (long long)v.x * (((unsigned)v.z + p - 1) / p) + (long long)v.y * (((unsigned)v.w + p - 1) / p);
+        }
+        const int need = __reduce_add_sync(0xffffffffu, (int)min(ctas * a.kv_heads, 1LL << 20));
+        if (lane == 0) sh.need[warp] = need;
+      }
+      __syncthreads();
+      int k = 0;
+      while (k < 8 && sh.need[k] > (int)gridDim.x) k++;
+      if (k < 8) {
+        cut.per += k;
+        cut.whole = true;
+        u = u > 0 ? units<NS>(a, q, cut) : 0;
+        total = block_sum(u, before);
+      }
+    }
+    share0 = min(total, cut.per * blockIdx.x);
+    share1 = min(total, share0 + cut.per);
     long long sum = 0;
     for (int i0 = 0; i0 < a.n; i0 += kTaThreads) {
       const int i = i0 + tid;
       long long all = total;
       if (a.n > kTaThreads) {  // otherwise the sums above stand
         if (i < a.n) q = request<KT>(a, i);
-        u = i < a.n ? units(a, q) : 0;
+        u = i < a.n ? units<NS>(a, q, cut) : 0;
         all = block_sum(u, before);
       }
       before += sum;
@@ -516,7 +575,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (blockIdx.x == 0 && i < a.n) parts.start[i] = before;
       sum += all;
     }
-    if (blockIdx.x == 0 && tid == 0) parts.start[a.n] = total, parts.start[a.n + 1] = per;
+    if (blockIdx.x == 0 && tid == 0) parts.start[a.n] = total, parts.start[a.n + 1] = cut.whole ? -cut.per : cut.per;
   }
   fence_before();
   __syncthreads();
@@ -536,6 +595,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     Walk<HD, Q> walk;
     walk.x0 = walk.x = share0;
     walk.x1 = share1;
+    walk.cut = cut;
     if (share0 < share1) walk.i = sh.req, walk.base = sh.base, walk.q = sh.q;
     Run run;
     auto hand_over = [&]() {
@@ -1041,19 +1101,24 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
   const int group = a.heads / a.kv_heads;
   pdl_wait();
   pdl_trigger();
-  if (head >= a.heads || r >= min(a.row_start[a.n], a.rows)) return;
-  const long long per = parts.start[a.n + 1];
+  const int last = a.row_start[a.n];
+  const long long signed_per = parts.start[a.n + 1], per = signed_per < 0 ? -signed_per : signed_per;
+  if (head >= a.heads || r >= min(last, a.rows)) return;
+  const Cut cut = {per, signed_per < 0};
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (a.row_start[mid + 1] > r) hi = mid;
     else lo = mid + 1;
   }
+  const long long start = parts.start[lo];
   const Req q = request<S::KT>(a, lo);
   const int kvh = head / group, m = (r - q.row0) * group + head - kvh * group;
   const int qt0 = m / 128 / S::NS * S::NS, w = min(S::NS, q.qt - qt0), wt = m & 127;
   if (w < 1 || m < 0) return;
-  const long long g0 = parts.start[lo] + (long long)kvh * q.qt * q.kt + (long long)qt0 * q.kt;
+  const Groups<S::NS> g(q, cut);
+  const long long g0 = start + kvh * g.all +
+                       (w == 2 ? qt0 / 2 * g.pair : g.pairs * g.pair + (qt0 - 2 * g.pairs) * g.single);
   const long long g1 = g0 + (long long)w * q.kt;
   const int c0 = (int)quot(g0, per), c1 = (int)quot(g1 - 1, per);
   // parts: both streams of each CTA of the group, or the query tile's own
@@ -1067,14 +1132,15 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
     const long long s = max((long long)c * per, g0), e1 = min((long long)(c + 1) * per, g1);
     const int ta = (int)((s - g0) >> (w - 1)), tb = (int)((e1 - g0) >> (w - 1));
     const bool ok = p < np && tb > ta && (w == 2 || t < tb - ta);
-    failed |= __any_sync(0xffffffffu, p < np && parts.status[min(c, ctas - 1)] != 0);
+    const size_t at = (((size_t)c * 2 + ((long long)c * per >= g0 ? 0 : 1)) * 2 + t) * parts.prow + wt;
+    const int status = p < np ? parts.status[min(c, ctas - 1)] : 0;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (ok) ml = *reinterpret_cast<const float2*>(parts.ml + at * 2);
+    failed |= __any_sync(0xffffffffu, status != 0);
     if (__any_sync(0xffffffffu, ok && ta == 0 && tb == q.kt)) {  // one CTA had it all and wrote the row
       if (!failed) return;
       break;
     }
-    const size_t at = (((size_t)c * 2 + ((long long)c * per >= g0 ? 0 : 1)) * 2 + t) * parts.prow + wt;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (ok) ml = *reinterpret_cast<const float2*>(parts.ml + at * 2);
     float top = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
