@@ -515,6 +515,25 @@ def test_attention_repeats_exactly():
         assert torch.equal(first, call_attention(a))
 
 
+@pytest.mark.parametrize("hd,repeats", [(64, 512), (128, 256), (256, 128)])
+def test_attention_f32_keeps_its_precision_over_long_contexts(hd, repeats):
+    """Tensor products cut their sums off: each addition loses up to 2^-23 of O,
+    always towards zero.  No more than 64 may go by before O is added up with
+    rounding, so the result is off by 64 x 2^-23 at most for those, whatever the
+    context's length, and by 2^-20 for the words of q and P and the scores.  The
+    context is 8,192 keys over and over, so its softmax is theirs."""
+    a = make_attention(21, [8192], [1], 2, 1, hd, F32)
+    a["q"] /= 4 * math.sqrt(hd / 64)
+    pages = a["tables"][0, :512]
+    k, v = (c[torch.as_tensor(pages, device="cuda")][:, 0].reshape(-1, hd).double() for c in (a["ck"], a["cv"]))
+    want = torch.softmax(a["q"][0].double() @ k.T / math.sqrt(hd), -1) @ v
+    # the row's own token is left out, so that the pages are all there is
+    b = dict(a, tables=np.concatenate([np.tile(pages, repeats), [-1]])[None], lengths=np.array([8192 * repeats]),
+             pos=np.array([8192 * repeats]), mask=np.zeros_like(a["mask"]))
+    got = call_attention(b)[0].double()
+    assert (got - want).norm() <= (64 * 2.0 ** -23 + 2.0 ** -20) * want.norm()
+
+
 @pytest.mark.parametrize("qt", [F32, BF16])
 def test_attention_many_requests(qt):
     """More requests than a CTA has threads."""

@@ -13,8 +13,9 @@
 // all of them.  A work item is a run of key tiles for one or two query tiles;
 // the key tiles of all (request, KV head, query tiles) are laid end to end and
 // cut evenly over one CTA per SM, whatever the lengths, each CTA finding its
-// share from a prefix sum over the requests.  A run that is not a whole group
-// leaves unnormalised parts (o, m, l), which k_tree_combine merges.
+// share from a prefix sum over the requests (where it costs little, so that no
+// CTA has parts of two groups).  A run that is not a whole group leaves
+// unnormalised parts (o, m, l), which k_tree_combine merges.
 //   a warp     brings K and V tiles in with TMA, a 16-token page at a time
 //              (its 64-column halves land in 128-byte-swizzled rows);
 //   a warp     issues S = Q K^T into TMEM and O += P V (P from TMEM, V as the
@@ -31,8 +32,27 @@
 // that it stays clear of both ends of the type; both factors cancel in o / l.
 // f32 queries enter as two f16 words (22 bits), and so does P, two products
 // each against the f16 cache; f16 and bf16 queries take P in their own type.
+// Tensor products cut their sums off instead of rounding them, so O loses up to
+// 2^-23 of itself, always towards zero, with each one added.  After 64 of them
+// (f32; 512 for the 16-bit types) it is added, in f32 with rounding, to a copy in
+// the workspace and starts again from zero: the error does not grow with the
+// context.  f32, 27 requests of 3 tokens over 19,360 keys: 1.8e-6 of the result in
+// 238 us, 1.3e-6 in 257 with 32, 2.8e-6 with 128, and 1.2e-5 in 219 without.
 // V rows of keys that no row may see (the end of the last page, a drafted node
 // that is left out) are zeroed in shared memory, since 0 * NaN is not 0.
+//
+// Measured: 8 requests of one token over 32,768 keys, 8 KV heads of 128: 1.07 GB
+// in 208 us = 5.2 TB/s, 80% of the measured copy rate.  32 trees of up to 64
+// tokens over 8,192 keys, 64 / 8 heads of 128, bf16: 414 GFLOP in 755 us = 548
+// TFLOP/s, 32% of the measured GEMM rate.  That is bound by latency: a stream goes
+// scores -> registers -> P -> product -> next scores with TMEM's 512 columns full
+// (two S, two O), so a pair of 128 x 128 tiles takes about 5,000 cycles, of which
+// the tensor pipe works 2,050 and the special-function unit (two exponentials per
+// score pair) 2,100.  Tried and slower: 64-key tiles with two S buffers per stream
+// (the products of 64 columns cost as much as those of 128), a thread per row with
+// its 128 scores in registers, P taken before the maximum is known, a product warp
+// per stream (both streams' exponentials then fall together), and a third of the
+// exponentials as polynomials on the FMA pipe.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -152,6 +172,8 @@ struct Shape {
   static constexpr int kFit = (kTaSmem - kQBytes - 3072) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
   static constexpr int kTiles = kQBytes + kSlots * kSlot;
+  // tiles after which O moves out of TMEM: 64 or 512 products
+  static constexpr int kFlush = (kSplit ? 64 : 512) / (KT / 16 * (kSplit ? 2 : 1));
   static constexpr int kO = 256;                       // TMEM column of O; S buffers from 0
   static constexpr bool kBf16 = std::is_same<Q, __nv_bfloat16>::value;
   static constexpr float kShift = kBf16 ? 0.f : 8.f;   // log2 of P's scale
@@ -366,9 +388,9 @@ struct Run {
   int i, kvh, qt0;
   int first, whole;   // the CTA's first run; the whole group
 };
-// Runs in flight: the TMA warp is ahead by no more than the ring's tiles, two
-// or more to a run, the others by one run.
-constexpr int kRuns = 8;
+// Runs in flight: the ring's 12 tiles are those of six runs at most, one more
+// waits for a slot, and the softmax may still be at the end of the one before.
+constexpr int kRuns = 9;
 
 // Walks the CTA's share [x, x1) of the laid-out key tiles; all threads alike.
 template <int HD, class Q>
@@ -436,6 +458,20 @@ __host__ inline Parts parts_at(void* ws, int ctas, int n, int hd, int prow) {
 }
 
 __device__ __forceinline__ void st4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+// O on its way out of TMEM, 16 columns of a row: a warp's rows side by side,
+// four columns of each after another, in the place of their parts
+__device__ __forceinline__ void put_kept(float* p, int rows, const float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) st4(p + e * 4 * rows, v + 4 * e);
+}
+__device__ __forceinline__ void add_kept(float* v, const float* p, int rows, float x) {
+  float4 y[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) y[e] = *reinterpret_cast<const float4*>(p + e * 4 * rows);
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    v[4 * e] += y[e].x * x, v[4 * e + 1] += y[e].y * x, v[4 * e + 2] += y[e].z * x, v[4 * e + 3] += y[e].w * x;
+}
 
 template <int HD, class Q>
 struct Small {  // behind the tiles in shared memory
@@ -532,7 +568,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     // A CTA that gets the end of one group and the start of the next pays a run's
     // fixed latency twice (about 6 us, as much as six units).  If there is a share
     // up to seven units larger with which every group has CTAs of its own, it is
-    // taken: 5 drafted tokens over 640 keys, 32 KV heads: 21 -> 16 us.
+    // taken (5 drafted tokens over 640 keys, 32 KV heads: last CTA done after 12.4
+    // instead of 15.7 us; 16 trees of 13 over 2048 keys: 30 instead of 33 us a call).
     if (a.n <= kTaThreads && cut.per < 4096) {
       // a warp per candidate, over the requests' groups (in the query tiles' place)
       int4* req = reinterpret_cast<int4*>(sm);
@@ -874,7 +911,13 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       // keys [open0, open1) are seen by all of the warp's rows
       int open0 = live ? pos < 0 || holes ? INT_MAX : a.window > 0 ? pos - a.window + 1 : 0 : 0;
       open0 = __reduce_max_sync(0xffffffffu, open0);
-      float mx = -INFINITY, l = 0.f;
+      // the place of the row's part, and of what O leaves there before
+      auto part = [&]() { return (((size_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * 2 + t) * parts.prow + wt; };
+      auto kept_rows = [&]() { return min(32, parts.prow - (wt & ~31)); };
+      auto keep = [&](int k) {
+        return parts.o + (part() - lane) * HD + ((hf * OW / 4 + 4 * k) * kept_rows() + lane) * 4;
+      };
+      float mx = -INFINITY, l = 0.f, m_kept = 0.f;  // m_kept: the maximum that belongs to what lies there
       const int step = NS == 2 ? 2 : 1;
       for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step, no++) {
         const int b = u & 1, v = NS == 2 ? 0 : b;
@@ -920,19 +963,32 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             mx = top;
             l *= scale;
           }
-          if (__any_sync(0xffffffffu, scale != 1.f)) {
+          const int done = u / step;  // the stream's tiles before this one
+          const bool flush = done > 0 && done % S::kFlush == 0;
+          if (flush || __any_sync(0xffffffffu, scale != 1.f)) {
             // O is at rest once the stream's last product is done (the one before it is: these scores came after)
             if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
             fence_after();
+            const float old = m_kept == mx ? 1.f : ex2(m_kept - mx);
 #pragma unroll 1
             for (int k = 0; k < OW / 16; k++) {
-              uint32_t v[16];
-              tm_ld16(op + k * 16, v);
-              tm_wait_ld16(v);
+              float v[16];
+              tm_ld16(op + k * 16, reinterpret_cast<uint32_t*>(v));
+              tm_wait_ld16(reinterpret_cast<uint32_t*>(v));
 #pragma unroll
-              for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
-              tm_st16(op + k * 16, v);
+              for (int e = 0; e < 16; e++) v[e] *= scale;
+              if (flush) {
+                if (live && wt < parts.prow) {
+                  if (done > S::kFlush) add_kept(v, keep(k), kept_rows(), old);
+                  put_kept(keep(k), kept_rows(), v);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 16; e++) v[e] = 0.f;
+              }
+              tm_st16(op + k * 16, reinterpret_cast<const uint32_t*>(v));
             }
+            if (flush) m_kept = mx;
           }
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
           const f2 c2 = make_f2(c, c), off2 = make_f2(off, off);
@@ -1019,11 +1075,26 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (ok) meet();
         if (!ok) break;
       }
+      if (warp_live && (nu - 1 - (NS == 2 ? t : 0)) / step >= S::kFlush) {
+        // O whole again; the halves' parts lie in one another's places
+        const float old = m_kept == mx ? 1.f : ex2(m_kept - mx);
+#pragma unroll 1
+        for (int k = 0; k < OW / 16; k++) {
+          float v[16];
+          tm_ld16(op + k * 16, reinterpret_cast<uint32_t*>(v));
+          tm_wait_ld16(reinterpret_cast<uint32_t*>(v));
+          if (live && wt < parts.prow) add_kept(v, keep(k), kept_rows(), old);
+          __syncwarp();
+          tm_st16(op + k * 16, reinterpret_cast<const uint32_t*>(v));
+        }
+        tm_wait_st();
+        meet();
+        if (!ok) break;
+      }
       float* po = nullptr;
       if (!run.whole && live && wt < parts.prow) {
-        const size_t at = (((size_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * 2 + t) * parts.prow + wt;
-        po = parts.o + at * HD + hf * OW;
-        if (hf == 0) *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(mx, l);
+        po = parts.o + part() * HD + hf * OW;
+        if (hf == 0) *reinterpret_cast<float2*>(parts.ml + part() * 2) = make_float2(mx, l);
       }
       Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD + hf * OW;
       const bool write = run.whole && live && !(merge && t == 1);
