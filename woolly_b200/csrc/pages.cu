@@ -10,7 +10,9 @@
 //
 // Both are prefix sums over the requests (one CTA, 1024 requests a round, sums
 // in 64 bits) and a scatter over the rows, which starts from a binary search of
-// the rows' prefix sums.
+// the rows' prefix sums.  Latency is all there is to them: 64 requests of one
+// token 4.0 us, 32 trees of up to 64 tokens 9.3 us, 1024
+// prompts of 314,000 rows 8.2 us (graph replays).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,7 +30,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanRows = 4096;  // rows that the scan's CTA places itself
+constexpr int kPlanRows = 2048;  // rows that the scan's CTA places itself
 
 __device__ __forceinline__ long long pages_of(long long tokens) { return (tokens + kKvPage - 1) / kKvPage; }
 
@@ -334,7 +336,9 @@ __device__ __forceinline__ uint4 to_cache(const Eight<C>& e) {
   return e.a;
 }
 
-// One thread moves eight values of K and of V.
+// One thread moves eight values of K and of V.  Bound by memory: 16 rows of 32
+// heads of 128 take 1.6 us in a graph (latency), 16 prompts of 512 rows of 8 heads
+// 8.6 us = 4.6 TB/s over the rows they have.
 template <class S, class C>
 __global__ void __launch_bounds__(256) k_kv_append(const S* k, const S* v, size_t ldk, size_t ldv,
                                                    const int* slots, int rows, int kvh, int hd, int n_slots,
@@ -406,8 +410,10 @@ int append_t(const void* k, const void* v, size_t ldk, size_t ldv, const int* sl
 
 }  // namespace
 
-// The rows join the scan's CTA while there are few of them; past that the
-// scatter takes a launch of its own over the whole GPU.
+// The rows join the scan's CTA while there are few of them; past that the scatter
+// takes a launch of its own over the whole GPU.  Graph replays, one launch and two:
+// 64 rows 4.2 and 6.2 us, 1,024 7.2 and 8.0, 2,048 9.9 and 8.5 (but a second launch
+// costs the host 2 us), 4,096 12.5 and 9.3.
 int launch_block_tables(const PlanArgs& a, cudaStream_t st) {
   const bool one = a.rows <= kPlanRows && a.n <= kPlanThreads;
   WL_TRY(launch_step(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, one ? 1 : 0));
