@@ -299,9 +299,8 @@ __global__ void __launch_bounds__(kLT, 2) k_logits(const LogitArgs a, int per) {
 template <class T>
 int launch_t(const LogitArgs& a, cudaStream_t st) {
   // drafted rows share their request's history: a CTA counts it once for up to
-  // eight, as many as leave two CTAs per SM.  Rows of 128,000 / 32,000: 512 of them
-  // take 118 / 39 us with eight and 304 / - with one; of 32,000, 128 take 27 us with
-  // two, 28 with one, 48 with eight.
+  // eight, as many as leave two CTAs per SM.  384 rows of 128,000 take 118 us with
+  // eight, 304 with one; 128 of 32,000 take 27 us with two, 28 with one, 48 with eight.
   const int runs = (a.vocab + kLChunk - 1) / kLChunk;
   int per = a.ctx.draft_mask ? kLRows : 1;
   while (per > 1 && (long long)((a.rows + per - 1) / per) * runs < 2 * 148) per /= 2;

@@ -169,7 +169,7 @@ struct Shape {
   static constexpr int kQTile = 128 * HD * 2;          // bytes of a query tile (one word)
   static constexpr int kQBytes = kQTile * NS * (kSplit ? 2 : 1);
   static constexpr int kSlot = KT * HD * 2;            // bytes of a K or V tile
-  static constexpr int kFit = (kTaSmem - kQBytes - 3072) / kSlot;
+  static constexpr int kFit = (kTaSmem - kQBytes - 3 * 1024) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
   static constexpr int kTiles = kQBytes + kSlots * kSlot;
   // tiles after which O moves out of TMEM: 64 or 512 products
