@@ -337,8 +337,8 @@ __device__ __forceinline__ uint4 to_cache(const Eight<C>& e) {
 }
 
 // One thread moves eight values of K and of V.  Bound by memory: 16 rows of 32
-// heads of 128 take 1.6 us in a graph (latency), 16 prompts of 512 rows of 8 heads
-// 8.6 us = 4.6 TB/s over the rows they have.
+// heads of 128 take 1.6 us in a graph (latency), 16 prompts of up to 512 rows of 8
+// heads (50 MB) 9.1 us a call = 5.5 TB/s, 85% of the measured copy rate.
 template <class S, class C>
 __global__ void __launch_bounds__(256) k_kv_append(const S* k, const S* v, size_t ldk, size_t ldv,
                                                    const int* slots, int rows, int kvh, int hd, int n_slots,
