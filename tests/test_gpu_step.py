@@ -534,6 +534,35 @@ def test_attention_f32_keeps_its_precision_over_long_contexts(hd, repeats):
     assert (got - want).norm() <= (64 * 2.0 ** -23 + 2.0 ** -20) * want.norm()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_f32_several_groups_per_cta(hd):
+    """Whole groups, and both ends of cut ones, in one CTA, each long enough
+    for O to leave TMEM on the way; single query tiles and pairs."""
+    rng = np.random.default_rng(hd)
+    counts = rng.choice([1, 5, 40, 70], 80)
+    a = make_attention(22, rng.integers(900, 2500, 80), counts, 8, 4, hd, F32)
+    close(call_attention(a), *ref_attention(a))
+
+
+@pytest.mark.parametrize("qt", [F16, BF16])
+@pytest.mark.parametrize("n,repeats", [(160, 4), (3, 400)])
+def test_attention_16_bit_long_contexts(qt, n, repeats):
+    """Requests over the same 8,192 keys, several times each: within a rounding
+    of the result and of P, and 512 cut-off additions (512 x 2^-23 = 2^-14)."""
+    hd, width = 64, 512 * repeats
+    a = make_attention(23, [8192], [1], 2, 1, hd, qt)
+    pages = a["tables"][0, :512]
+    k, v = (c[torch.as_tensor(pages, device="cuda")][:, 0].reshape(-1, hd).double() for c in (a["ck"], a["cv"]))
+    w = torch.softmax(a["q"][0].double() @ k.T / math.sqrt(hd), -1)
+    want, size = w @ v, w @ v.abs()
+    b = dict(a, tables=np.tile(np.concatenate([np.tile(pages, repeats), [-1]]), (n, 1)),
+             lengths=np.full(n, 16 * width), start=np.arange(n + 1), pos=np.full(n, 16 * width),
+             mask=np.zeros((n, 1), np.uint32), rows=n, q=a["q"].expand(n, 2, hd).contiguous())
+    got = call_attention(b).double()
+    tol = HALF[qt] * want.abs() + (HALF[qt] + 2.0 ** -14) * size
+    assert ((got - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("qt", [F32, BF16])
 def test_attention_many_requests(qt):
     """More requests than a CTA has threads."""

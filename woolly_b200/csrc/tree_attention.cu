@@ -33,17 +33,18 @@
 // f32 queries enter as two f16 words (22 bits), and so does P, two products
 // each against the f16 cache; f16 and bf16 queries take P in their own type.
 // Tensor products cut their sums off instead of rounding them, so O loses up to
-// 2^-23 of itself, always towards zero, with each one added.  After 64 of them
+// 2^-23 of itself, always towards zero, with each one added.  After 32 of them
 // (f32; 512 for the 16-bit types) it is added, in f32 with rounding, to a copy in
-// the workspace and starts again from zero: the error does not grow with the
-// context.  f32, 27 requests of 3 tokens over 19,360 keys: 1.8e-6 of the result in
-// 238 us, 1.3e-6 in 257 with 32, 2.8e-6 with 128, and 1.2e-5 in 219 without.
+// the workspace and starts again from zero, while the next scores are on their way:
+// the error does not grow with the context.  f32, 27 requests of 3 tokens over
+// 19,360 keys: 1.3e-6 of the result in 237 us, 1.8e-6 in 226 with 64, 1.2e-5 in 219
+// without.
 // V rows of keys that no row may see (the end of the last page, a drafted node
 // that is left out) are zeroed in shared memory, since 0 * NaN is not 0.
 //
 // Measured: 8 requests of one token over 32,768 keys, 8 KV heads of 128: 1.07 GB
-// in 208 us = 5.2 TB/s, 80% of the measured copy rate.  32 trees of up to 64
-// tokens over 8,192 keys, 64 / 8 heads of 128, bf16: 414 GFLOP in 755 us = 548
+// in 206 us = 5.2 TB/s, 81% of the measured copy rate.  32 trees of up to 64
+// tokens over 8,192 keys, 64 / 8 heads of 128, bf16: 414 GFLOP in 742 us = 557
 // TFLOP/s, 32% of the measured GEMM rate.  That is bound by latency: a stream goes
 // scores -> registers -> P -> product -> next scores with TMEM's 512 columns full
 // (two S, two O), so a pair of 128 x 128 tiles takes about 5,000 cycles, of which
@@ -172,8 +173,8 @@ struct Shape {
   static constexpr int kFit = (kTaSmem - kQBytes - 3 * 1024) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
   static constexpr int kTiles = kQBytes + kSlots * kSlot;
-  // tiles after which O moves out of TMEM: 64 or 512 products
-  static constexpr int kFlush = (kSplit ? 64 : 512) / (KT / 16 * (kSplit ? 2 : 1));
+  // tiles after which O moves out of TMEM: 32 or 512 products
+  static constexpr int kFlush = (kSplit ? 32 : 512) / (KT / 16 * (kSplit ? 2 : 1));
   static constexpr int kO = 256;                       // TMEM column of O; S buffers from 0
   static constexpr bool kBf16 = std::is_same<Q, __nv_bfloat16>::value;
   static constexpr float kShift = kBf16 ? 0.f : 8.f;   // log2 of P's scale
@@ -922,6 +923,30 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step, no++) {
         const int b = u & 1, v = NS == 2 ? 0 : b;
         const int tile = pair ? u >> 1 : u, key0 = first + tile * KT;
+        const int done = u / step;  // the stream's tiles before this one
+        if (done > 0 && done % S::kFlush == 0 && warp_live) {
+          // O leaves TMEM while the next scores are on their way, once it is at rest.  The
+          // scores seen so far came after the product before the last (two streams), or
+          // the one before that (one): a wait may not be a phase further ahead.
+          if (NS == 1 && !(ok = wait_warp(obar + 8 * t, (no - 2) & 1))) break;
+          if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
+          fence_after();
+          const float old = m_kept == mx ? 1.f : ex2(m_kept - mx);
+          m_kept = mx;
+#pragma unroll 1
+          for (int k = 0; k < OW / 16; k++) {
+            float v[16];
+            tm_ld16(op + k * 16, reinterpret_cast<uint32_t*>(v));
+            tm_wait_ld16(reinterpret_cast<uint32_t*>(v));
+            if (live && wt < parts.prow) {
+              if (done > S::kFlush) add_kept(v, keep(k), kept_rows(), old);
+              put_kept(keep(k), kept_rows(), v);
+            }
+            __syncwarp();
+            const uint32_t zero[16] = {};
+            tm_st16(op + k * 16, zero);
+          }
+        }
         ok = wait_warp(sbar + 8 * b, ns >> v & 1);
         ns ^= 1u << v;
         if (!ok) break;
@@ -963,32 +988,19 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             mx = top;
             l *= scale;
           }
-          const int done = u / step;  // the stream's tiles before this one
-          const bool flush = done > 0 && done % S::kFlush == 0;
-          if (flush || __any_sync(0xffffffffu, scale != 1.f)) {
+          if (__any_sync(0xffffffffu, scale != 1.f)) {
             // O is at rest once the stream's last product is done (the one before it is: these scores came after)
             if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
             fence_after();
-            const float old = m_kept == mx ? 1.f : ex2(m_kept - mx);
 #pragma unroll 1
             for (int k = 0; k < OW / 16; k++) {
-              float v[16];
-              tm_ld16(op + k * 16, reinterpret_cast<uint32_t*>(v));
-              tm_wait_ld16(reinterpret_cast<uint32_t*>(v));
+              uint32_t v[16];
+              tm_ld16(op + k * 16, v);
+              tm_wait_ld16(v);
 #pragma unroll
-              for (int e = 0; e < 16; e++) v[e] *= scale;
-              if (flush) {
-                if (live && wt < parts.prow) {
-                  if (done > S::kFlush) add_kept(v, keep(k), kept_rows(), old);
-                  put_kept(keep(k), kept_rows(), v);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int e = 0; e < 16; e++) v[e] = 0.f;
-              }
-              tm_st16(op + k * 16, reinterpret_cast<const uint32_t*>(v));
+              for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
+              tm_st16(op + k * 16, v);
             }
-            if (flush) m_kept = mx;
           }
           const float off = (mx == -INFINITY ? 0.f : -mx) + S::kShift;
           const f2 c2 = make_f2(c, c), off2 = make_f2(off, off);
