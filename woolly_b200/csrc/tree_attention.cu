@@ -923,12 +923,12 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       for (int u = NS == 2 ? t : 0; u < nu && (NS == 2 || t == 0); u += step, no++) {
         const int b = u & 1, v = NS == 2 ? 0 : b;
         const int tile = pair ? u >> 1 : u, key0 = first + tile * KT;
+        if (NS == 1 && !(ok = wait_warp(sbar + 8 * b, ns >> v & 1))) break;
         const int done = u / step;  // the stream's tiles before this one
         if (done > 0 && done % S::kFlush == 0 && warp_live) {
-          // O leaves TMEM while the next scores are on their way, once it is at rest.  The
-          // scores seen so far came after the product before the last (two streams), or
-          // the one before that (one): a wait may not be a phase further ahead.
-          if (NS == 1 && !(ok = wait_warp(obar + 8 * t, (no - 2) & 1))) break;
+          // O leaves TMEM once it is at rest, while the next scores are on their way.  The
+          // wait must be for the phase that may still be open: scores seen before came
+          // after the product before the last.  With one stream that takes these scores.
           if (!(ok = wait_warp(obar + 8 * t, (no - 1) & 1))) break;
           fence_after();
           const float old = m_kept == mx ? 1.f : ex2(m_kept - mx);
@@ -947,9 +947,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             tm_st16(op + k * 16, zero);
           }
         }
-        ok = wait_warp(sbar + 8 * b, ns >> v & 1);
+        if (NS == 2 && !(ok = wait_warp(sbar + 8 * b, ns >> v & 1))) break;
         ns ^= 1u << v;
-        if (!ok) break;
         fence_after();
         const uint32_t sp = tmem + lanes + b * KT + hf * CW;
         if (warp_live) {
