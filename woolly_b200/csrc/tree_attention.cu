@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   }
   const uint32_t full = sptr(sh.bars), empty = full + 8 * NSLOT, qbar = empty + 8 * NSLOT, sbar = qbar + 8,
                  pbar = sbar + 32, dbar = pbar + 32, obar = dbar + 8, endbar = obar + 16, xfull = endbar + 8,
-                 xempty = xfull + 16, hbar = xempty + 16, rbar = hbar + 64;
+                 xempty = xfull + 16, hbar = xempty + 16, rbar = hbar + 64, mbar = rbar + 8 * kRuns;
   const uint32_t qs = sptr(sm), ring = qs + S::kQBytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.heads / a.kv_heads;
@@ -525,6 +525,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     for (int k = 0; k < kRuns; k++) bar_init(rbar + 8 * k, 1);
     bar_init(dbar, 1);
     bar_init(endbar, 1);
+    bar_init(mbar, kTaSoft);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     sh.fail = 0;
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mk) : "memory");
@@ -1163,8 +1164,14 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
         }
       }
-      // the exchange's last round has been read before its place is written again
-      if (merge && t == 1 && ok) ok = wait_warp(xempty + 8 * hf, (nx - 1) & 1);
+      // All warps have read the exchange's last round, and the other stream's (m, l),
+      // before any of them copies the next run's queries: a pair's second query tile
+      // takes the exchange's place.
+      if (merge) {
+        if (!ok) break;
+        arrive_warp(mbar);
+        if (!(ok = wait_warp(mbar, (nx / (OW / 16) - 1) & 1))) break;  // nx: OW / 16 a merge
+      }
     }
   }
   fence_before();
