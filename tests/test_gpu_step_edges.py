@@ -34,3 +34,23 @@ def test_single_query_tiles_before_pairs(qt, hd):
     close(first, *ref_attention(a))
     for _ in range(40):
         assert torch.equal(call_attention(a), first)
+
+
+@pytest.mark.parametrize("hd,keys,step", [(64, 128, 3.5), (128, 128, 3.5), (256, 64, 7.0)])
+@pytest.mark.parametrize("counts", [[1], [20, 5], [70]])
+def test_the_maximum_rises_where_o_leaves_tmem(hd, keys, step, counts):
+    """Scores that rise by 2^7 from one key tile of a stream to its next (`step`
+    doublings every `keys` keys), past the lag of 2^6: O is rescaled at every
+    tile, those at which it has just left TMEM among them.  What O held before
+    then weighs 2^-7, and V lies around 1, so an O that counts twice shows as
+    0.8% of the result; the bound is below 0.3%."""
+    a = make_attention(32, [1024] * len(counts), counts, 4, 1, hd, F32)
+    a["q"] *= 0.25
+    a["q"][..., 0] = math.sqrt(hd)                       # so that k[0] adds to the score as it is
+    a["cv"] += 1
+    for i in range(len(counts)):
+        for p in range(1024 // P):
+            a["ck"][a["tables"][i, p], :, :, 0] = p * P // keys * step * math.log(2.0)
+    want, tol = ref_attention(a)
+    assert float((tol / want.abs()).median()) < 3e-3
+    close(call_attention(a), want, tol)

@@ -947,6 +947,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             const uint32_t zero[16] = {};
             tm_st16(op + k * 16, zero);
           }
+          tm_wait_st();  // a rescale of the same tile reads the zeros
         }
         if (NS == 2 && !(ok = wait_warp(sbar + 8 * b, ns >> v & 1))) break;
         ns ^= 1u << v;
