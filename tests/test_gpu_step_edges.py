@@ -54,3 +54,37 @@ def test_the_maximum_rises_where_o_leaves_tmem(hd, keys, step, counts):
     want, tol = ref_attention(a)
     assert float((tol / want.abs()).median()) < 3e-3
     close(call_attention(a), want, tol)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 0.01, 1e5, 1e30])
+def test_f32_queries_of_any_size(hd, size):
+    """q times `size` over a scale divided by it: the scores are what they were,
+    and q keeps its 22 bits, far outside of f16's range too."""
+    a = make_attention(33, [300, 40, 700], [3, 70, 1], 8, 2, hd, F32)
+    a["q"] *= size
+    close(call_attention(a, scale=hd ** -0.5 / size), *ref_attention(a, scale=hd ** -0.5 / size))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_f32_queries_of_many_sizes_in_a_call(hd):
+    """Heads of large queries over small keys and the reverse, rows of zeros,
+    and one element far above the others of its row; several runs in a CTA."""
+    counts = [70, 1, 40, 130] * 5
+    a = make_attention(34, [200] * 20, counts, 32, 8, hd, F32)
+    for h in range(8):
+        a["q"][:, 4 * h:4 * h + 4] *= 2.0 ** (3 * h - 9)
+        a["ck"][:, h] *= 2.0 ** (9 - 3 * h)
+    a["q"][::7] = 0
+    a["q"][3::5, ::3, 11] = 3e5
+    a["ck"][:, :, :, 11] = 0
+    want, tol = ref_attention(a)
+    # The row is scaled so that its largest value lies in [2^14, 2^15).  There the
+    # first f16 word leaves at most 2^-11 of an element; the second holds that to
+    # 2^-11 of it (22 bits, which ref_attention counts) or, where it falls among f16's
+    # subnormals, to half of their step, 2^-25, which is at most 2^-39 of the largest.
+    # A score is off by that times the sum of |k|, twice that moves the normaliser too.
+    k = a["ck"].double().abs().sum(-1).amax(dim=(0, 2)).repeat_interleave(4)  # per head
+    big = a["q"].double().abs().amax(-1)
+    tol += (2 * 2.0 ** -39 * hd ** -0.5 * big * k * a["cv"].double().abs().max())[..., None]
+    close(call_attention(a), want, tol)

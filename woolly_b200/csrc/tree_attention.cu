@@ -30,8 +30,10 @@
 // The maximum that P is taken against follows the true one with a lag of up to
 // 2^6 (O is rescaled only past that), and P is scaled by 2^8 where it is f16, so
 // that it stays clear of both ends of the type; both factors cancel in o / l.
-// f32 queries enter as two f16 words (22 bits), and so does P, two products
-// each against the f16 cache; f16 and bf16 queries take P in their own type.
+// f32 queries enter as two f16 words, their rows scaled by a power of two that the
+// score factor takes back: 22 bits of each element, or 2^-39 of the row's largest
+// where that is more.  P too is two words (22 bits), two products each against the
+// f16 cache; f16 and bf16 queries take P in their own type.
 // Tensor products cut their sums off instead of rounding them, so O loses up to
 // 2^-23 of itself, always towards zero, with each one added.  After 32 of them
 // (f32; 512 for the 16-bit types) it is added, in f32 with rounding, to a copy in
@@ -795,7 +797,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t oth = hbar + 8 * (t * 4 + (warp & 3));  // meets the other half's warp
     const uint32_t op = tmem + lanes + S::kO + (NS == 2 ? t * HD : 0) + hf * OW;
-    const float c = a.scale * 1.4426950408889634f;
+    float c = a.scale * 1.4426950408889634f;
     uint32_t ns = 0, runs = 0, no = 0, seq = 0;  // ns: parities of the stream's S buffers; no: its products so far
     uint32_t nx = 0;           // exchanges between the streams
     uint32_t nh = 0;           // and between the halves
@@ -806,6 +808,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     auto arrive_warp = [&](uint32_t bar) {
       __syncwarp();
       if (lane == 0) bar_arrive(bar);
+    };
+    auto meet_all = [&](uint32_t parity) {  // all softmax warps
+      arrive_warp(mbar);
+      return wait_warp(mbar, parity & 1);
     };
     auto meet = [&]() {
       arrive_warp(oth);
@@ -825,6 +831,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (!__all_sync(0xffffffffu, rp != nullptr) || rp->nt == 0) break;
       const Run& run = *rp;
       const int nt = run.nt, pair = run.w == 2, nu = pair ? 2 * nt : nt, len = run.len, first = run.key0;
+      // f32: the rows' factors go through sh.half, which the run before may still be reading
+      if (S::kSplit && runs > 0 && !(ok = meet_all(runs - 1))) break;
       // queries: the threads copy 16-byte pieces of the (row, head) pairs
       {
         const int m0 = run.qt0 * 128, mn = min(run.w * 128, run.T * group - m0);
@@ -837,7 +845,20 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           uint8_t* d = sm + (m >> 7) * S::kQTile + (ch >> 3) * 128 * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
           if constexpr (S::kSplit) {
             const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
-            const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            // The row times a power of two that brings its largest value to 2^14 .. 2^15, clear
+            // of both ends of f16; the HD / 8 lanes that copy the row find it together.
+            uint32_t big = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) big = max(big, __float_as_uint(f[k]) & 0x7fffffffu);
+            constexpr int LR = HD / 8;
+            big = __reduce_max_sync((LR == 32 ? 0xffffffffu : (1u << (LR & 31)) - 1) << (lane & ~(LR - 1)), big) >> 23;
+            const int up = big == 255 ? 0 : min(141 - (int)big, 100);  // the power; inf and NaN stay
+            const float factor = __uint_as_float((127 + up) << 23);
+#pragma unroll
+            for (int k = 0; k < 8; k++) f[k] *= factor;
+            // and its inverse for the threads of the row, each of which has a place of its own
+            if (ch < 4 && (!pair || ch >> 1 == m >> 7)) sh.half[ch >> 1][ch & 1][row] = __uint_as_float((127 - up) << 23);
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -856,6 +877,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       fence_async();
       fence_before();
       arrive_warp(qbar);
+      if constexpr (S::kSplit) {
+        if (!(ok = wait_warp(qbar, runs & 1))) break;
+        c = fmaxf(a.scale * 1.4426950408889634f * sh.half[NS == 2 ? t : 0][hf][wt], 0x1p-126f);  // -inf * c stays -inf
+      }
 
       const int m = (run.qt0 + (pair ? t : 0)) * 128 + wt;
       const int j = m / group, g = m - j * group;
@@ -1167,12 +1192,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       }
       // All warps have read the exchange's last round, and the other stream's (m, l),
       // before any of them copies the next run's queries: a pair's second query tile
-      // takes the exchange's place.
-      if (merge) {
-        if (!ok) break;
-        arrive_warp(mbar);
-        if (!(ok = wait_warp(mbar, (nx / (OW / 16) - 1) & 1))) break;  // nx: OW / 16 a merge
-      }
+      // takes the exchange's place.  (f32: they meet before every run.)
+      if (!ok) break;
+      if (!S::kSplit && merge && !(ok = meet_all(nx / (OW / 16) - 1))) break;  // nx: OW / 16 a merge
     }
   }
   fence_before();
