@@ -88,3 +88,26 @@ def test_f32_queries_of_many_sizes_in_a_call(hd):
     big = a["q"].double().abs().amax(-1)
     tol += (2 * 2.0 ** -39 * hd ** -0.5 * big * k * a["cv"].double().abs().max())[..., None]
     close(call_attention(a), want, tol)
+
+
+def token(a, cache, i, t):
+    """All heads of token t of request i in a cache."""
+    return a[cache][a["tables"][i, t // P], :, t % P]
+
+
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 129])
+def test_nothing_below_the_window_is_felt(qt, hd, window):
+    """inf and NaN in K and V right below every row's window, and values of the
+    largest size further below, leave the result as it is."""
+    a = make_attention(35, [300, 515, 40], [3, 70, 1], 4, 2, hd, qt)
+    want, tol = ref_attention(a, window)
+    big = torch.finfo(a["ck"].dtype).max
+    for i, n in enumerate(a["lengths"]):
+        for t in range(n - window + 1):
+            for c in ("ck", "cv"):
+                token(a, c, i, t)[:] = (math.nan, math.inf, -math.inf, big, -big)[t % 5] if n - window - t < 40 else big
+    close(call_attention(a, window), want, tol)
+    close(call_attention(a, window, masked=False), *ref_attention(
+        dict(a, ck=a["ck"].nan_to_num(0, 0, 0), cv=a["cv"].nan_to_num(0, 0, 0)), window, masked=False))

@@ -42,7 +42,8 @@
 // 19,360 keys: 1.3e-6 of the result in 237 us, 1.8e-6 in 226 with 64, 1.2e-5 in 219
 // without.
 // V rows of keys that no row may see (the end of the last page, a drafted node
-// that is left out) are zeroed in shared memory, since 0 * NaN is not 0.
+// that is left out, cached tokens below the window) are zeroed in shared memory,
+// since 0 * NaN is not 0.
 //
 // Measured: 8 requests of one token over 32,768 keys, 8 KV heads of 128: 1.07 GB
 // in 206 us = 5.2 TB/s, 81% of the measured copy rate.  32 trees of up to 64
@@ -1059,9 +1060,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           l += lo_of(sum[0]) + hi_of(sum[0]);
           tm_wait_st();
         }
-        if (hf == 0 && key0 + KT > len) {
-          // V rows that no row sees: keys past the end, nodes in nobody's mask.
-          // A warp takes 32 keys, its lanes the request's rows.
+        if (hf == 0 && (key0 + KT > len || (a.window > 0 && key0 <= len - a.window))) {
+          // V rows that no row sees: keys past the end, nodes in nobody's mask, cached
+          // tokens below every row's window.  A warp takes 32 keys, its lanes the
+          // request's rows.
           const int k0 = key0 + (wt & ~31);
           bool dead = false;
           if (wt < KT) {
@@ -1077,7 +1079,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
               seen = __reduce_or_sync(0xffffffffu, seen);
               if (k0 < len) seen |= (1u << (len - k0)) - 1u;  // cached tokens of the word
             }
-            dead = key0 + wt >= run.keys || !(seen >> lane & 1u);
+            dead = key0 + wt >= run.keys || !(seen >> lane & 1u) || (a.window > 0 && key0 + wt <= len - a.window);
           }
           const uint32_t k = seq + (uint32_t)(min(nt, tile + (pair ? NB / 2 : NB)) + tile);
           const uint32_t slot = k % NSLOT;
