@@ -111,3 +111,61 @@ def test_nothing_below_the_window_is_felt(qt, hd, window):
     close(call_attention(a, window), want, tol)
     close(call_attention(a, window, masked=False), *ref_attention(
         dict(a, ck=a["ck"].nan_to_num(0, 0, 0), cv=a["cv"].nan_to_num(0, 0, 0)), window, masked=False))
+
+
+def spoil(a, window, masked, where):
+    """Puts inf, -inf and NaN into single columns of V at the tokens `where`
+    [(request, node)] and gives, from the definition, the outputs that are not
+    finite then: a column of a row is the sum of what its row attends."""
+    rows, heads, hd = a["q"].shape
+    out = torch.zeros(rows, heads, hd, dtype=torch.float64, device="cuda")
+    G = heads // a["cv"].shape[1]
+    for n, (i, c) in enumerate(where):
+        L, r0 = int(a["lengths"][i]), int(a["start"][i])
+        d = (5 * n + 3) % hd
+        bad = (math.inf, -math.inf, math.nan, math.inf)[n % 4]
+        token(a, "cv", i, L + c)[:, d] = bad
+        for j in range(int(a["start"][i + 1]) - r0):
+            r = r0 + j
+            if c < 0:
+                see, at = True, L + c
+            else:
+                see = bool(a["mask"][r, c // 32] >> np.uint32(c % 32) & 1) if masked else c <= j
+                at = a["pos"][r0 + c]
+            if see and (window == 0 or at > a["pos"][r] - window):
+                out[r, :, d] += bad
+    return out
+
+
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("shape", ["trees", "chains", "window", "many", "long"])
+def test_what_is_not_finite_stays_with_the_rows_that_attend_it(qt, hd, shape):
+    """inf and NaN in V of drafted tokens, later tokens of a prompt and tokens that
+    only some rows have in their window reach the rows that attend them, as the
+    sum says, and no others: runs of one CTA, parts of several, pairs of query
+    tiles and merged streams."""
+    window, masked, where = 0, True, None
+    if shape == "trees":
+        a = make_attention(36, [40, 300, 0], [20, 70, 5], 8, 2, hd, qt)
+        where = [(0, 3), (0, 17), (1, 2), (1, 40), (1, 69), (2, 4)]
+    elif shape == "chains":
+        a, masked = make_attention(37, [0, 130], [150, 90], 4, 1, hd, qt, tree="chain"), False
+        where = [(0, 60), (0, 140), (1, 1), (1, 89)]
+    elif shape == "window":
+        a, window = make_attention(38, [200, 333], [40, 9], 4, 2, hd, qt, tree="chain"), 100
+        where = [(0, -95), (0, -60), (1, -97), (1, -92), (0, 3)]
+    elif shape == "many":  # more groups than SMs: whole ones, several to a CTA
+        a = make_attention(39, [100 + 9 * i for i in range(40)], [1 + 7 * (i % 11) for i in range(40)], 16, 4, hd, qt)
+        where = [(i, (3 * i) % (1 + 7 * (i % 11))) for i in range(0, 40, 3)]
+    else:
+        a = make_attention(40, [5000], [6], 8, 1, hd, qt)
+        where = [(0, 2), (0, 5)]
+    want, tol = ref_attention(a, window, masked)
+    plus = spoil(a, window, masked, where)
+    got = call_attention(a, window, masked)
+    odd = ~plus.isfinite()
+    assert 0 < int(odd.sum()) < odd.numel() // 4
+    assert torch.equal(got[odd].double().nan_to_num(nan=7.0), plus[odd].nan_to_num(nan=7.0))
+    close(got.masked_fill(odd, 0), want.masked_fill(odd, 0), tol)
+    assert torch.equal(got.nan_to_num(nan=7.0), call_attention(a, window, masked).nan_to_num(nan=7.0))

@@ -435,8 +435,9 @@ struct Walk {
 
 // Parts: [CTA][first / last run][stream][prow rows][HD] f32, then (m, l) of
 // each; one status word per CTA and the requests' prefix sums before them.
+constexpr int kGaveUp = 1, kOdd = 2;  // a wait ran out; some O is not finite
 struct Parts {
-  int* status;       // [ctas]
+  int* status;       // [ctas] bits
   long long* start;  // [n] prefix sums, then the total and a CTA's share (negative: whole groups)
   float* o;
   float* ml;
@@ -488,7 +489,7 @@ struct Small {  // behind the tiles in shared memory
   };
   long long base;
   Req q;
-  int req, fail, need[8];
+  int req, fail, odd, need[8];
   uint32_t tmem;
 };
 
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     bar_init(endbar, 1);
     bar_init(mbar, kTaSoft);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    sh.fail = 0;
+    sh.fail = sh.odd = 0;
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mk) : "memory");
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(&mv) : "memory");
   }
@@ -1138,6 +1139,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       }
       Q* out = (Q*)a.out + ((size_t)row * a.heads + (size_t)run.kvh * group + g) * HD + hf * OW;
       const bool write = run.whole && live && !(merge && t == 1);
+      f2 odd[2] = {make_f2(0.f, 0.f), make_f2(0.f, 0.f)};  // 0 * O: NaN where O is not finite
 #pragma unroll 1
       for (int k = 0; k < OW / 16; k++) {
         float v[16];
@@ -1167,6 +1169,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
           nx++;
         }
+        if (po || write) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) odd[e & 1] = fma2(make_f2(v[2 * e], v[2 * e + 1]), make_f2(0.f, 0.f), odd[e & 1]);
+        }
         if (po) {
 #pragma unroll
           for (int e = 0; e < 16; e += 4) st4(po + k * 16 + e, v + e);
@@ -1192,6 +1198,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
         }
       }
+      odd[0] = add2(odd[0], odd[1]);
+      if (lo_of(odd[0]) + hi_of(odd[0]) != 0.f) sh.odd = 1;  // NaN is unequal too
       // All warps have read the exchange's last round, and the other stream's (m, l),
       // before any of them copies the next run's queries: a pair's second query tile
       // takes the exchange's place.  (f32: they meet before every run.)
@@ -1202,15 +1210,81 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   fence_before();
   __syncthreads();
   if (warp == kTaSoft + kTaLoad) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
-  if (tid == 0) parts.status[blockIdx.x] = sh.fail;
+  if (tid == 0) parts.status[blockIdx.x] = (sh.fail ? kGaveUp : 0) | (sh.odd ? kOdd : 0);
+}
+
+// One (row, head) by the definition, a warp in f32, 32 keys at a time: the keys that
+// the row does not attend are not touched.
+template <int HD, class Q>
+__device__ __noinline__ void row_again(const TreeAttnArgs& a, int i, int r, int head, float* s_q) {
+  const Req q = request<Shape<HD, Q>::KT>(a, i);
+  using C = typename std::conditional<Shape<HD, Q>::kSplit, __half, Q>::type;
+  const int lane = threadIdx.x & 31, kvh = head / (a.heads / a.kv_heads);
+  const int pos = a.pos[r] < 0 ? -1 : max(a.pos[r], q.len), end = pos < 0 ? 0 : q.keys;
+  const Q* src = (const Q*)a.q + (size_t)r * a.ldq + (size_t)head * HD;
+#pragma unroll
+  for (int e = 0; e < HD / 32; e++) s_q[e * 32 + lane] = as_f32(src[e * 32 + lane]);
+  __syncwarp();
+  float m = -INFINITY, l = 0.f, o[HD / 32] = {};
+  for (int t0 = q.tile0 * Shape<HD, Q>::KT; t0 < end; t0 += 32) {
+    const int t = t0 + lane, c = t - q.len;
+    bool see = t < end;
+    if (see && c >= 0)
+      see = a.mask ? c < 32 * a.words && (a.mask[(size_t)r * a.words + (c >> 5)] >> (c & 31) & 1u) : c <= r - q.row0;
+    if (see && a.window > 0) see = (c >= 0 ? max(a.pos[q.row0 + c], q.len) : t) > pos - a.window;
+    const int page = see ? a.tables[(size_t)i * a.ld_tables + t / kKvPage] : -1;
+    see = page >= 0 && page < a.n_pages;
+    const size_t at = see ? (((size_t)page * a.kv_heads + kvh) * kKvPage + t % kKvPage) * HD : 0;
+    float s = -INFINITY;
+    if (see) {
+      const uint4* k = reinterpret_cast<const uint4*>((const C*)a.cache_k + at);
+      float acc = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < HD / 8; d++) {
+        const uint4 u = k[d];
+        const C* x = reinterpret_cast<const C*>(&u);
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc += s_q[d * 8 + e] * as_f32(x[e]);
+      }
+      s = acc * a.scale;
+    }
+    float mn = s;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+    mn = fmaxf(m, mn);
+    const float old = m == -INFINITY ? 0.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);
+    float sum = p, part[HD / 32] = {};
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    for (unsigned todo = __ballot_sync(0xffffffffu, p != 0.f); todo; todo &= todo - 1) {
+      const float pk = __shfl_sync(0xffffffffu, p, __ffs(todo) - 1);
+      const C* v = (const C*)a.cache_v + __shfl_sync(0xffffffffu, at, __ffs(todo) - 1) + lane;
+#pragma unroll
+      for (int e = 0; e < HD / 32; e++) part[e] += pk * as_f32(v[e * 32]);
+    }
+    l = l * old + sum;
+    m = mn;
+#pragma unroll
+    for (int e = 0; e < HD / 32; e++) o[e] = o[e] * old + part[e];
+  }
+  Q* out = (Q*)a.out + ((size_t)r * a.heads + head) * HD + lane;
+#pragma unroll
+  for (int e = 0; e < HD / 32; e++) put(out + e * 32, l == 0.f ? 0.f : o[e] / l);
 }
 
 // Merges the parts of the groups that were cut: a warp per (row, head), its
 // lanes a part each for the weights, then HD / 32 columns each.  A row of a call
 // in which a CTA's wait gave up becomes NaN.
+// A product takes every key of its tiles for every row, those that a row does not
+// attend with P = 0.  inf or NaN in the V of one that another row does attend (a
+// sibling in the tree, a later token of the chain, a token that only shallower rows
+// have in their window) makes that 0 * NaN, so a row that comes out other than
+// finite is worked out again without them (row_again).  That costs nothing where
+// all is finite: the main kernel's CTAs say whether they saw anything else.
 template <int HD, class Q>
-__global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, const Parts parts, int ctas) {
+__global__ void __launch_bounds__(128) k_tree_combine(const __grid_constant__ TreeAttnArgs a, const Parts parts, int ctas) {
   using S = Shape<HD, Q>;
+  __shared__ float s_q[4][HD];
   const int lane = threadIdx.x & 31, r = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
   const int group = a.heads / a.kv_heads;
   pdl_wait();
@@ -1237,7 +1311,7 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
   const int c0 = (int)quot(g0, per), c1 = (int)quot(g1 - 1, per);
   // parts: both streams of each CTA of the group, or the query tile's own
   const int nt = w == 2 ? 1 : S::NS, np = (c1 - c0 + 1) * nt;
-  bool failed = false;
+  bool failed = false, odd = false, whole = false;
   float M = -INFINITY, L = 0.f, o[HD / 32];
 #pragma unroll
   for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
@@ -1250,9 +1324,11 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
     const int status = p < np ? parts.status[min(c, ctas - 1)] : 0;
     float2 ml = make_float2(-INFINITY, 0.f);
     if (ok) ml = *reinterpret_cast<const float2*>(parts.ml + at * 2);
-    failed |= __any_sync(0xffffffffu, status != 0);
+    failed |= __any_sync(0xffffffffu, status & kGaveUp);
+    odd |= __any_sync(0xffffffffu, status & kOdd);
     if (__any_sync(0xffffffffu, ok && ta == 0 && tb == q.kt)) {  // one CTA had it all and wrote the row
-      if (!failed) return;
+      if (!failed && !odd) return;
+      whole = true;
       break;
     }
     float top = ml.y == 0.f ? -INFINITY : ml.x;
@@ -1280,6 +1356,16 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeAttnArgs a, cons
     }
   }
   Q* out = (Q*)a.out + ((size_t)r * a.heads + head) * HD;
+  if (odd && !failed) {
+    bool again = false;
+#pragma unroll
+    for (int e = 0; e < HD / 32; e++) again |= !isfinite(whole ? as_f32(out[e * 32 + lane]) : L == 0.f ? 0.f : o[e]);
+    if (__any_sync(0xffffffffu, again) && !(whole && a.q == a.out)) {  // in place the query is gone
+      row_again<HD, Q>(a, lo, r, head, s_q[threadIdx.x >> 5]);
+      return;
+    }
+    if (whole) return;
+  }
 #pragma unroll
   for (int e = 0; e < HD / 32; e++) put(out + e * 32 + lane, failed ? NAN : L == 0.f ? 0.f : o[e] / L);
 }
