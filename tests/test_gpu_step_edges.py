@@ -169,3 +169,31 @@ def test_what_is_not_finite_stays_with_the_rows_that_attend_it(qt, hd, shape):
     assert torch.equal(got[odd].double().nan_to_num(nan=7.0), plus[odd].nan_to_num(nan=7.0))
     close(got.masked_fill(odd, 0), want.masked_fill(odd, 0), tol)
     assert torch.equal(got.nan_to_num(nan=7.0), call_attention(a, window, masked).nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_scores_that_are_not_finite_show(qt, hd):
+    """NaN in a query or in an attended key, and a score of inf, give NaN as the
+    softmax does, and no zeros; -inf scores weigh nothing, a masked key's NaN too."""
+    a = make_attention(41, [0, 70, 300], [4, 30, 1], 4, 2, hd, qt)
+    a["q"][2, 1, 5] = math.nan                     # one row of one head
+    token(a, "ck", 1, 70 + 4)[0, 7] = math.nan     # node 4 of request 1, KV head 0
+    token(a, "ck", 2, 11)[1, 0] = math.inf         # all of request 2's rows, KV head 1: heads 2 and 3
+    r = int(a["start"][2])
+    a["q"][r, :, 0] = a["q"][r, :, 0].abs() + 1
+    a["q"][r, 3, 0] *= -1                          # head 3: the score is -inf
+    nan = torch.zeros(a["rows"], 4, dtype=torch.bool, device="cuda")
+    nan[2, 1] = True
+    for j in range(30):
+        if a["mask"][4 + j, 0] >> np.uint32(4) & 1:
+            nan[4 + j, :2] = True
+    nan[r, 2] = True
+    b = dict(a, q=a["q"].nan_to_num(0), ck=a["ck"].clone())
+    token(b, "ck", 1, 74)[0, 7] = 0
+    token(b, "ck", 2, 11)[1, 0] = torch.finfo(a["ck"].dtype).max  # head 3: a weight of 0 all the same
+    want, tol = ref_attention(b)
+    tol[r, 3] = tol[:r].amax()  # that score's size is none of the others'
+    got = call_attention(a)
+    assert torch.equal(got.isnan().all(-1), nan) and torch.equal(got.isnan().any(-1), nan)
+    close(got.masked_fill(nan[..., None], 0), want.masked_fill(nan[..., None], 0), tol)

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
     __syncthreads();
   }
   Q* out = (Q*)a.out + ((size_t)r * a.heads + head) * hd;
-  for (int e = 0, d = tid; d < hd; d += 128, e++) put(out + d, l > 0.f ? o[e] / l : 0.f);
+  for (int e = 0, d = tid; d < hd; d += 128, e++) put(out + d, l == 0.f ? 0.f : o[e] / l);
 }
 
 
