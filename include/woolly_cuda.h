@@ -277,7 +277,9 @@ int wl_swiglu(const float* gate, const float* up, size_t n, float* out, void* st
  * top-p keeps nothing when no prefix exceeds p, as the reference), then
  * greedy (temperature == 0: last index of the largest probability) or the
  * first index whose running sum exceeds the row's uniform draw u (last index
- * when none does).  params and out_ids are device arrays of `rows` entries;
+ * when none does, and greedily where nothing is kept: the last whose logit is
+ * not -inf, so that a token that a mask closed is not returned while another is
+ * open).  params and out_ids are device arrays of `rows` entries;
  * vocab <= 51200.  The draw is an input: the caller owns the random stream. */
 typedef struct wl_sample_params {
   float temperature;

@@ -11,6 +11,10 @@
 //   temperature == 0: the last index of the largest prob
 //   else: the first index whose running sum (index order) exceeds a uniform
 //     draw u in [0, 1); the last index when none does.
+// A token whose logit is -inf is closed (a grammar's mask) and never returned while
+// another one is open: where the rules above leave nothing to choose from (no
+// running sum exceeds the draw, top-p keeps nothing), the last index is that of the
+// last open token, and it is the vocabulary's last when none is closed.
 // The uniform draw of each row is an input, so the host keeps the random
 // stream (one per request).
 //
@@ -289,6 +293,16 @@ __global__ void __launch_bounds__(kST) k_sample(const float* logits, int V, int 
       for (int i = j0; i < j1; i++) ps_[pad(i)] = ps_[pad(i)] / ps;
   }
 
+  struct IMax {
+    __device__ int operator()(int a, int b) const { return a > b ? a : b; }
+  };
+  auto last_open = [&]() {  // all threads
+    int last = -1;
+    for (int i = tid; i < V; i += kST)
+      if (x[i] != -INFINITY) last = i;
+    last = block_reduce(last, IMax(), redi);
+    return last < 0 ? V - 1 : last;
+  };
   if (P.temperature == 0.0f) {
     // greedy: the last index of the largest prob (Rust max_by keeps the last)
     unsigned long long best = 0;
@@ -297,7 +311,10 @@ __global__ void __launch_bounds__(kST) k_sample(const float* logits, int V, int 
       best = best > key ? best : key;
     }
     best = block_reduce(best, ArgMaxLast(), redu);
-    if (tid == 0) out[r] = (uint32_t)(best & 0xFFFFFFFFu);
+    int pick = (int)(best & 0xFFFFFFFFu);
+    const float p = __uint_as_float((uint32_t)(best >> 32));
+    if (!(p > 0.f)) pick = last_open();  // nothing kept, or NaN
+    if (tid == 0) out[r] = (uint32_t)pick;
     return;
   }
   // inverse CDF in index order (inference.rs:638-654)
@@ -307,8 +324,10 @@ __global__ void __launch_bounds__(kST) k_sample(const float* logits, int V, int 
   int hit = V;
   float run = base;
   for (int i = j0; i < j1; i++) {
+    // a prob of zero is no hit: `base`, summed in another order than the thread before
+    // this one did, may already exceed a draw that its own sums did not
     run += ps_[pad(i)];
-    if (run > P.u) {
+    if (ps_[pad(i)] > 0.f && run > P.u) {
       hit = i;
       break;
     }
@@ -317,7 +336,8 @@ __global__ void __launch_bounds__(kST) k_sample(const float* logits, int V, int 
     __device__ int operator()(int a, int b) const { return a < b ? a : b; }
   };
   hit = block_reduce(hit, IMin(), redi);
-  if (tid == 0) out[r] = (uint32_t)(hit < V ? hit : V - 1);
+  if (hit == V) hit = last_open();
+  if (tid == 0) out[r] = (uint32_t)hit;
 }
 
 }  // namespace

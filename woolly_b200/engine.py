@@ -15,6 +15,9 @@ apply_top_p_filtering: inference.rs:551-630): temperature floor 0.01, top-k
 by the k-th largest probability, top-p by the first prefix whose cumulative
 probability exceeds p, greedy (temperature == 0) as the last index of the
 largest probability, and a stop on token ids below 3 (inference.rs:414-418).
+Where they leave nothing to choose from, the reference takes the last index;
+here it is the last whose logit is not -inf, so that a closed token is never
+picked.
 
 Before sampling, a request's logits may go through rules that the reference
 does not have: penalties for tokens that its prompt or output holds, biases and
@@ -100,17 +103,26 @@ def sample_next_token(logits: np.ndarray, cfg: GenerationConfig, rng: np.random.
         probs = apply_top_p(probs, cfg.top_p)
     if cfg.temperature == 0.0:
         m = probs.max()
-        return int(np.flatnonzero(probs == m)[-1])  # Rust max_by keeps the last maximum
-    return sample_from_distribution(probs, rng)
+        # Rust max_by keeps the last maximum; zero (top-p kept nothing) and NaN are none
+        return int(np.flatnonzero(probs == m)[-1]) if m > 0 else last_open(logits)
+    return sample_from_distribution(probs, rng, logits)
 
 
-def sample_from_distribution(probs: np.ndarray, rng: np.random.Generator) -> int:
+def last_open(logits: np.ndarray) -> int:
+    """The last index whose logit is not -inf (of a row without one, the last)."""
+    i = np.flatnonzero(np.asarray(logits) != -np.inf)
+    return int(i[-1]) if i.size else len(logits) - 1
+
+
+def sample_from_distribution(probs: np.ndarray, rng: np.random.Generator,
+                             logits: np.ndarray | None = None) -> int:
     """inference.rs:638-654: first index whose f32 running sum exceeds a
-    uniform draw in [0, 1); the last index when none does (e.g. all zeros)."""
+    uniform draw in [0, 1); the last index when none does (e.g. all zeros), of
+    those that `logits` leaves open."""
     u = np.float32(rng.random(dtype=np.float32))
     cum = np.cumsum(probs, dtype=np.float32)
     hit = np.flatnonzero(cum > u)
-    return int(hit[0]) if hit.size else probs.size - 1
+    return int(hit[0]) if hit.size else last_open(probs if logits is None else logits)
 
 
 def allowed_mask(cfg: GenerationConfig, tokens, vocab: int) -> np.ndarray | None:
