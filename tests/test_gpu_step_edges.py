@@ -197,3 +197,28 @@ def test_scores_that_are_not_finite_show(qt, hd):
     got = call_attention(a)
     assert torch.equal(got.isnan().all(-1), nan) and torch.equal(got.isnan().any(-1), nan)
     close(got.masked_fill(nan[..., None], 0), want.masked_fill(nan[..., None], 0), tol)
+
+
+def test_engine_biases_that_close_on_the_gpu(tiny_models):
+    """Biases of -inf, with and without a grammar, end or steer a request alike
+    on the host and on the GPU."""
+    from woolly_b200.engine import BatchEngine, GenerationConfig
+    from woolly_b200.model import CudaTransformer
+    shut = {t: -math.inf for t in range(0, 1000, 2)}
+    cfgs = [GenerationConfig(max_tokens=8, eos_below=0, temperature=0.9, seed=3, logit_bias=shut),
+            GenerationConfig(max_tokens=8, eos_below=0, logit_bias=shut, allowed=lambda t: range(len(t), 300)),
+            GenerationConfig(max_tokens=8, eos_below=0, logit_bias=shut,
+                             allowed=lambda t: [4, 6, 7] if len(t) < 3 else [4, 6]),
+            GenerationConfig(max_tokens=8, eos_below=0)]
+    runs = []
+    for dev in (False, True):
+        m = CudaTransformer(tiny_models["gqa_q4_0"], max_sessions=4, max_context=64, max_batch=4)
+        eng = BatchEngine(m, device_sampling=dev)
+        ids = [eng.submit([5, 6, 7 + i], c) for i, c in enumerate(cfgs)]
+        eng.run()
+        runs.append([(eng.finished[i].tokens, eng.finished[i].reason) for i in ids])
+        eng.close()
+        m.close()
+    assert runs[0] == runs[1]
+    assert all(t % 2 or t >= 1000 for toks, _ in runs[0][:3] for t in toks)
+    assert runs[0][2] == ([7, 7, 7], "constraint") and len(runs[0][0][0]) == 8

@@ -45,7 +45,7 @@ class GenerationConfig:
     repetition_penalty: float = 1.0  # logits of seen tokens: divided if positive, else multiplied (1: off)
     presence_penalty: float = 0.0    # taken off the logits of produced tokens, once
     frequency_penalty: float = 0.0   # and once for each time that they were produced
-    logit_bias: dict | None = None   # token id -> added to its logit
+    logit_bias: dict | None = None   # token id -> added to its logit; below -1e38 (-inf) the token is closed
     # callable(tokens produced so far) -> ids that may follow, a boolean mask over the
     # vocabulary, or None for any; an empty answer ends the request ("constraint")
     allowed: object = None
@@ -125,6 +125,20 @@ def sample_from_distribution(probs: np.ndarray, rng: np.random.Generator,
     return int(hit[0]) if hit.size else last_open(probs if logits is None else logits)
 
 
+RULE_MAX = 1e30     # penalties and biases of at most this leave logits finite in f32
+BIAS_CLOSED = -1e38  # biases below this close their token
+
+
+def open_mask(cfg: GenerationConfig, tokens, vocab: int) -> np.ndarray | None:
+    """allowed_mask without the tokens that a bias closes."""
+    m = allowed_mask(cfg, tokens, vocab)
+    closed = [t for t, b in (cfg.logit_bias or {}).items() if b < BIAS_CLOSED]
+    if closed:
+        m = np.ones(vocab, bool) if m is None else m.copy()
+        m[closed] = False
+    return m
+
+
 def allowed_mask(cfg: GenerationConfig, tokens, vocab: int) -> np.ndarray | None:
     """Boolean mask of the ids that may follow `tokens`, or None when any may."""
     if cfg.allowed is None:
@@ -158,8 +172,9 @@ def apply_rules(logits: np.ndarray, cfg: GenerationConfig, prompt, tokens,
     x[seen] = np.where(x[seen] > 0, x[seen] / r, x[seen] * r)
     hit = made > 0
     x[hit] -= np.float32(cfg.frequency_penalty) * made[hit].astype(np.float32) + np.float32(cfg.presence_penalty)
-    for t, b in (cfg.logit_bias or {}).items():
-        x[t] += np.float32(b)
+    with np.errstate(over="ignore"):  # a bias below f32's range is -inf
+        for t, b in (cfg.logit_bias or {}).items():
+            x[t] += np.float32(b)
     if mask is not None:
         x[~mask] = -np.inf
     return x
@@ -190,8 +205,9 @@ def pack_rules(requests, masks, vocab: int) -> dict:
         history=flat(hist, np.int32), history_start=starts(hist),
         prompt_lens=np.asarray([len(r.prompt) for r in requests], np.int32))
     if any(bias):
-        out.update(bias_start=starts(bias), bias_tokens=flat([[t for t, _ in b] for b in bias], np.int32),
-                   bias_values=flat([[v for _, v in b] for b in bias], np.float32))
+        with np.errstate(over="ignore"):
+            out.update(bias_start=starts(bias), bias_tokens=flat([[t for t, _ in b] for b in bias], np.int32),
+                       bias_values=flat([[v for _, v in b] for b in bias], np.float32))
     if words:
         out["allowed"] = np.stack(words)
     return out
@@ -220,8 +236,9 @@ class BatchEngine:
     token), then decodes one token for every other running request in one
     batched forward; run() steps until every request has finished.  A request
     finishes after cfg.max_tokens tokens, on a token id below cfg.eos_below,
-    when its session's context is full, or when its grammar allows nothing.  Its session is released at once,
-    so a waiting request can take the slot on the next step.
+    when its session's context is full, or when its grammar and its biases leave no
+    token open ("constraint").  Its session is released at once, so a waiting
+    request can take the slot on the next step.
     """
 
     def __init__(self, model, max_batch: int | None = None, session_factory=None,
@@ -252,13 +269,13 @@ class BatchEngine:
         if not prompt:
             raise ValueError("empty prompt (the reference's EMPTY_INPUT)")
         cfg = cfg or GenerationConfig()
-        if not (np.isfinite(cfg.repetition_penalty) and cfg.repetition_penalty > 0):
-            raise ValueError("repetition_penalty must be positive and finite")
-        if not (np.isfinite(cfg.presence_penalty) and np.isfinite(cfg.frequency_penalty)):
-            raise ValueError("presence_penalty and frequency_penalty must be finite")
+        if not (1 / RULE_MAX <= cfg.repetition_penalty <= RULE_MAX):
+            raise ValueError(f"repetition_penalty must lie in [{1 / RULE_MAX}, {RULE_MAX}]")
+        if not (abs(cfg.presence_penalty) <= RULE_MAX and abs(cfg.frequency_penalty) <= RULE_MAX):
+            raise ValueError(f"presence_penalty and frequency_penalty must lie within +-{RULE_MAX}")
         for t, b in (cfg.logit_bias or {}).items():
-            if not (0 <= t < self.model.vocab_size()) or np.isnan(b):
-                raise ValueError(f"logit_bias: token {t} outside the vocabulary, or not a number")
+            if not (0 <= t < self.model.vocab_size()) or not b <= RULE_MAX:
+                raise ValueError(f"logit_bias: token {t} outside the vocabulary, or its bias not up to {RULE_MAX}")
         r = Request(self._next, prompt, cfg, np.random.default_rng(cfg.seed), on_token=on_token)
         self._next += 1
         self.waiting.append(r)
@@ -267,7 +284,7 @@ class BatchEngine:
     # ---------------------------------------------------------------- internals
     def _mask(self, r: Request) -> np.ndarray | None:
         """The request's mask; one that leaves nothing ends the request."""
-        m = allowed_mask(r.cfg, r.tokens, self.model.vocab_size())
+        m = open_mask(r.cfg, r.tokens, self.model.vocab_size())
         if m is not None and not m.any():
             r.done, r.reason = True, "constraint"
         return m
