@@ -64,3 +64,98 @@ def test_submit_refuses_what_f32_cannot_hold(kw):
     m = FakeModel()
     with pytest.raises(ValueError):
         BatchEngine(m, session_factory=m.new_session).submit([1], GenerationConfig(**kw))
+
+
+class Stop(Exception):
+    pass
+
+
+def raises_at(n, ids=range(V)):
+    """A grammar that raises once n tokens are there."""
+    def allowed(tokens):
+        if len(tokens) == n:
+            raise Stop
+        return ids
+    return allowed
+
+
+def drain(eng):
+    """Steps until all is finished; the number of steps that raised."""
+    raised = 0
+    for _ in range(100):
+        if eng.idle():
+            return raised
+        try:
+            eng.step()
+        except Stop:
+            raised += 1
+    raise AssertionError("requests that never finish")
+
+
+@pytest.mark.parametrize("model,device", [(FakeModel, False), (DeviceModel, True)])
+@pytest.mark.parametrize("at", [0, 1, 3])
+def test_a_grammar_that_raises_ends_its_own_request(model, device, at):
+    """On the first token, where the request has just been admitted, or later:
+    the others' tokens are those of a run without it, and all sessions close."""
+    cfg = lambda **kw: GenerationConfig(max_tokens=6, eos_below=0, temperature=0.8, **kw)  # noqa: E731
+    prompts = [[3, 4], [8], [9, 9], [2, 7]]
+    alone = [run(model(), [p], [cfg(seed=i)], device_sampling=device)[0].tokens for i, p in enumerate(prompts)]
+    m = model()
+    eng = BatchEngine(m, session_factory=m.new_session, device_sampling=device)
+    ids = [eng.submit(p, cfg(seed=i, allowed=raises_at(at)) if i == 1 else cfg(seed=i))
+           for i, p in enumerate(prompts)]
+    assert drain(eng) == 1
+    assert m.open == 0
+    got = [eng.finished[i] for i in ids]
+    assert [r.tokens for i, r in enumerate(got) if i != 1] == [t for i, t in enumerate(alone) if i != 1]
+    assert got[1].reason == "error" and got[1].tokens == alone[1][:at]
+
+
+@pytest.mark.parametrize("model,device", [(FakeModel, False), (DeviceModel, True)])
+@pytest.mark.parametrize("at", [1, 2, 5])
+def test_a_callback_that_raises_costs_no_token(model, device, at):
+    seen = []
+
+    def callback(rid, tok, done, reason):
+        seen.append((rid, tok))
+        if rid == 0 and sum(r == 0 for r, _ in seen) == at:
+            raise Stop
+    m = model()
+    eng = BatchEngine(m, session_factory=m.new_session, device_sampling=device)
+    cfg = GenerationConfig(max_tokens=5, eos_below=0)
+    ids = [eng.submit([p], cfg, on_token=callback) for p in (3, 8)]
+    assert drain(eng) == 1 and m.open == 0
+    for i, p in zip(ids, (3, 8)):
+        want = run(model(), [[p]], [cfg])[0].tokens
+        assert eng.finished[i].tokens == want == [t for r, t in seen if r == i]
+        assert eng.finished[i].reason == "length"
+
+
+def test_a_prefill_that_raises_leaves_the_other_requests():
+    class Broken(FakeModel):
+        def forward_sessions(self, sessions, ids):
+            if any(13 in i for i in ids):
+                raise Stop
+            return super().forward_sessions(sessions, ids)
+    m = Broken()
+    eng = BatchEngine(m, session_factory=m.new_session)
+    cfg = GenerationConfig(max_tokens=3, eos_below=0, allowed=lambda t: [1, 2])
+    ids = [eng.submit(p, cfg) for p in ([13], [5], [6, 13], [7])]
+    assert drain(eng) == 1 and m.open == 0
+    assert [eng.finished[i].reason for i in ids] == ["error", "length", "error", "length"]
+
+
+def test_a_session_that_cannot_be_made_keeps_those_admitted():
+    m = FakeModel()
+
+    def factory():
+        if m.open == 1 and factory.broken:
+            factory.broken = False
+            raise Stop
+        return m.new_session()
+    factory.broken = True
+    eng = BatchEngine(m, session_factory=factory)
+    cfg = GenerationConfig(max_tokens=3, eos_below=0)
+    ids = [eng.submit([p], cfg) for p in (4, 5)]
+    assert drain(eng) == 1 and m.open == 0
+    assert [len(eng.finished[i].tokens) for i in ids] == [3, 3]

@@ -289,13 +289,8 @@ class BatchEngine:
             r.done, r.reason = True, "constraint"
         return m
 
-    def _emit(self, r: Request, row: np.ndarray) -> None:
-        ruled = row
-        if r.cfg.has_rules():
-            mask = self._mask(r)
-            if r.done:
-                return
-            ruled = apply_rules(row, r.cfg, r.prompt, r.tokens, mask)
+    def _emit(self, r: Request, row: np.ndarray, mask: np.ndarray | None) -> None:
+        ruled = apply_rules(row, r.cfg, r.prompt, r.tokens, mask) if r.cfg.has_rules() else row
         tok = sample_next_token(ruled, r.cfg, r.rng)
         if self.keep_logits:
             r.logits.append(np.array(row, np.float32, copy=True))
@@ -323,9 +318,9 @@ class BatchEngine:
                 keep.append(r)
         self.running = keep
 
-    def _admit(self) -> list[Request]:
-        new = []
-        while self.waiting and len(self.running) + len(new) < self.max_batch:
+    def _admit(self) -> None:
+        """Moves waiting requests to `running`, whose sessions the engine closes."""
+        while self.waiting and len(self.running) < self.max_batch:
             r = self.waiting[0]
             if self.max_context is not None and len(r.prompt) >= self.max_context:
                 self.waiting.pop(0)
@@ -339,47 +334,69 @@ class BatchEngine:
                     break
                 raise
             self.waiting.pop(0)
-            new.append(r)
-        return new
+            self.running.append(r)
 
     # ---------------------------------------------------------------- public
     def step(self) -> int:
-        """One scheduler iteration; returns the number of tokens produced."""
-        produced = 0
-        decoding = [r for r in self.running if not r.done]
-        new = self._admit()
-        for r in new:  # prefill: the prompt's last row gives the first token
-            row = self.model.forward_sessions([r.session], [r.prompt])[0]
-            self._emit(r, np.asarray(row).reshape(-1)[-self.model.vocab_size():])
-            produced += len(r.tokens)
-        if decoding and self.device_sampling:
-            kw = {}
-            if any(r.cfg.has_rules() for r in decoding):
-                masks = [self._mask(r) for r in decoding]
-                masks = [m for m, r in zip(masks, decoding) if not r.done]
-                decoding = [r for r in decoding if not r.done]
-                kw["rules"] = pack_rules(decoding, masks, self.model.vocab_size())
-        if decoding and self.device_sampling:
-            cf = [r.cfg for r in decoding]
-            u = [np.float32(r.rng.random(dtype=np.float32)) if r.cfg.temperature != 0.0 else 0.0
-                 for r in decoding]
-            toks = self.model.decode_sample([r.session for r in decoding],
-                                            [r.tokens[-1] for r in decoding],
-                                            [c.temperature for c in cf], [c.top_k for c in cf],
-                                            [c.top_p for c in cf], u, **kw)
-            for r, tok in zip(decoding, toks):
-                self._emit_token(r, tok)
-                produced += 1
-        elif decoding:
-            outs = self.model.forward_sessions([r.session for r in decoding],
-                                               [[r.tokens[-1]] for r in decoding])
-            for r, row in zip(decoding, outs):
-                n = len(r.tokens)
-                self._emit(r, np.asarray(row).reshape(-1))
-                produced += len(r.tokens) - n
-        self.running += new
-        self._retire()
+        """One scheduler iteration; returns the number of tokens produced.
+
+        An exception from a request's own part is raised once the others have
+        finished the step (the first, of several).  One from its grammar or its
+        prefill ends the request with the reason "error"; after one from on_token
+        it goes on, its token being produced."""
+        produced, errors = 0, []
+
+        def alone(r, part, *args):
+            n = len(r.tokens)
+            try:
+                return part(r, *args)
+            except Exception as e:
+                if len(r.tokens) == n:
+                    r.done, r.reason = True, "error"
+                errors.append(e)
+
+        decoding = [r for r in self.running if r.tokens]
+        try:
+            self._admit()
+            for r in self.running:  # prefill: the prompt's last row gives the first token
+                if not r.tokens:
+                    alone(r, self._prefill)
+                    produced += len(r.tokens)
+            # before anything is decoded, since a grammar may end its request or raise
+            masks = {r.rid: alone(r, self._mask) for r in decoding}
+            decoding = [r for r in decoding if not r.done]
+            if decoding and self.device_sampling:
+                kw = {}
+                if any(r.cfg.has_rules() for r in decoding):
+                    kw["rules"] = pack_rules(decoding, [masks[r.rid] for r in decoding], self.model.vocab_size())
+                cf = [r.cfg for r in decoding]
+                u = [np.float32(r.rng.random(dtype=np.float32)) if r.cfg.temperature != 0.0 else 0.0
+                     for r in decoding]
+                toks = self.model.decode_sample([r.session for r in decoding],
+                                                [r.tokens[-1] for r in decoding],
+                                                [c.temperature for c in cf], [c.top_k for c in cf],
+                                                [c.top_p for c in cf], u, **kw)
+                for r, tok in zip(decoding, toks):
+                    alone(r, self._emit_token, tok)
+                    produced += 1
+            elif decoding:
+                outs = self.model.forward_sessions([r.session for r in decoding],
+                                                   [[r.tokens[-1]] for r in decoding])
+                for r, row in zip(decoding, outs):
+                    n = len(r.tokens)
+                    alone(r, self._emit, np.asarray(row).reshape(-1), masks[r.rid])
+                    produced += len(r.tokens) - n
+        finally:
+            self._retire()
+        if errors:
+            raise errors[0]
         return produced
+
+    def _prefill(self, r: Request) -> None:
+        mask = self._mask(r)
+        if not r.done:
+            row = self.model.forward_sessions([r.session], [r.prompt])[0]
+            self._emit(r, np.asarray(row).reshape(-1)[-self.model.vocab_size():], mask)
 
     def idle(self) -> bool:
         return not self.waiting and not self.running
