@@ -222,3 +222,17 @@ def test_engine_biases_that_close_on_the_gpu(tiny_models):
     assert runs[0] == runs[1]
     assert all(t % 2 or t >= 1000 for toks, _ in runs[0][:3] for t in toks)
     assert runs[0][2] == ([7, 7, 7], "constraint") and len(runs[0][0][0]) == 8
+
+
+@pytest.mark.parametrize("n", [1, 1024, 1025, 3000])
+def test_block_tables_without_rows(n):
+    """Nothing to place: the lengths stay, requests that wanted rows are told."""
+    from woolly_b200 import STEP_NO_ROWS, STEP_OK
+    counts = np.zeros(n, int)
+    counts[-1] = 2
+    t = torch.full((n, 3), -1, dtype=torch.int32, device="cuda")
+    plan = ops.block_tables(t, i32(np.arange(n) % 40), i32(counts), i32([4, 5]), i32([2]), 0)
+    assert plan.status.tolist() == [STEP_OK] * (n - 1) + [STEP_NO_ROWS]
+    assert plan.lengths.tolist() == [i % 40 for i in range(n)] and plan.free_count.tolist() == [2]
+    assert plan.row_start.tolist() == [0] * (n + 1) and (t == -1).all()
+    assert plan.slots.numel() == plan.requests.numel() == plan.positions.numel() == 0

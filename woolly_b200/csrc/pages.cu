@@ -417,7 +417,7 @@ int append_t(const void* k, const void* v, size_t ldk, size_t ldv, const int* sl
 int launch_block_tables(const PlanArgs& a, cudaStream_t st) {
   const bool one = a.rows <= kPlanRows && a.n <= kPlanThreads;
   WL_TRY(launch_step(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, one ? 1 : 0));
-  if (!one) WL_TRY(launch_step(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a));
+  if (!one && a.rows > 0) WL_TRY(launch_step(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a));
   return WL_OK;
 }
 
