@@ -395,7 +395,8 @@ int wl_kv_commit(int cache_type, const int* tables, int ld_tables, int max_pages
  * negative position, and rows with nothing to attend, give zeros; rows behind
  * row_start[n] are left as they were.  Keys on pages outside the cache are
  * masked.  inf and NaN in K or V reach the rows that attend their token, no
- * others.  q and out are f32 over an f16 cache, or f16 / bf16 over a cache of
+ * others.  out may be q itself, with packed rows (inf and NaN in V then also reach
+ * other rows of the request); else it may not overlap it.  q and out are f32 over an f16 cache, or f16 / bf16 over a cache of
  * the same type; head_dim 32, 64, 128 or 256.  f32 queries may have any finite
  * size; at head_dim 64 and above they count with 22 bits of each element, or
  * 2^-39 of the row's largest where that is more.  workspace: wl_tree_attention_workspace

@@ -236,3 +236,15 @@ def test_block_tables_without_rows(n):
     assert plan.lengths.tolist() == [i % 40 for i in range(n)] and plan.free_count.tolist() == [2]
     assert plan.row_start.tolist() == [0] * (n + 1) and (t == -1).all()
     assert plan.slots.numel() == plan.requests.numel() == plan.positions.numel() == 0
+
+
+@pytest.mark.parametrize("qt", [F32, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_attention_in_place(qt, hd):
+    """The output on the queries: whole groups, cut ones, several in a CTA."""
+    for n, (lengths, counts, heads, kvh) in enumerate((([300, 20], [70, 3], 8, 2), ([4000], [5], 4, 1),
+                                                       ([130] * 40, [9, 70] * 20, 16, 4))):
+        a = make_attention(42 + n, lengths, counts, heads, kvh, hd, qt)
+        want = call_attention(a)
+        assert call_attention(a, out=a["q"]) is a["q"]
+        assert torch.equal(a["q"], want)

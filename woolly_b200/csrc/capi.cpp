@@ -511,6 +511,10 @@ int wl_attention(const float* q, const float* k, const float* v, int rows, int p
 
 // ---------------- a serving step on a paged cache ----------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + nq && b < a + np;
+}
 constexpr int kMaxTablePages = 1 << 26;  // tokens of a request stay below 2^30
 
 int wl_block_tables(int* tables, int ld_tables, int max_pages, const int* lengths, const int* counts, int n,
@@ -618,6 +622,10 @@ int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k
   if (!aligned16(q) || ldq * es % 16 || !aligned16(out) || !aligned16(cache_k) || !aligned16(cache_v) ||
       !aligned16(workspace))
     return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: q, out, caches and workspace must be 16-byte aligned");
+  const size_t width = (size_t)heads * head_dim;
+  if (!(out == q && ldq == width) &&
+      overlap(q, ((size_t)(rows - 1) * ldq + width) * es, out, (size_t)rows * width * es))
+    return fail(WL_ERR_INVALID_ARGUMENT, "tree_attention: out overlaps q (it may be q itself, with packed rows)");
   TreeAttnArgs a;
   a.q = q, a.ldq = ldq, a.q_type = q_type, a.cache_k = cache_k, a.cache_v = cache_v, a.n_pages = n_pages;
   a.tables = tables, a.ld_tables = ld_tables, a.max_pages = max_pages, a.lengths = lengths;

@@ -485,7 +485,8 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     `scale` defaults to head_dim ** -0.5.
     A row with a negative position or nothing to attend gives zeros; rows
     behind row_start[n] are not written.  q is f32 over an f16 cache, or has
-    the cache's type; head_dim 32, 64, 128 or 256."""
+    the cache's type; head_dim 32, 64, 128 or 256.  `out` may be a packed q,
+    else it may not overlap it."""
     index, pages, kvh, hd, ct = _caches(cache_k, cache_v)
     try:
         qt = q.dtype
