@@ -410,7 +410,7 @@ int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* Rules on logits before sampling, per row r of [rows][vocab] (f32, f16 or
- * bf16; row strides ld, ldo; out may be logits).  With n_v the times token v
+ * bf16; row strides ld, ldo; out may be logits, else no row of it may overlap one).  With n_v the times token v
  * occurs among the tokens that the row's request produced, and v "seen" when
  * it occurs there or in the prompt:
  *   y = seen ? (x > 0 ? x / repetition : x * repetition) : x

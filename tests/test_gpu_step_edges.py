@@ -248,3 +248,16 @@ def test_attention_in_place(qt, hd):
         want = call_attention(a)
         assert call_attention(a, out=a["q"]) is a["q"]
         assert torch.equal(a["q"], want)
+
+
+def test_logits_beside_their_output():
+    """Column ranges of one matrix, the output's on either side."""
+    for ld, x0, y0 in ((20, 0, 10), (20, 10, 0), (33, 11, 23), (33, 20, 2)):
+        m = torch.randn(6, ld, device="cuda")
+        x, y = m[:, x0:x0 + 10], m[:, y0:y0 + 10]
+        prm = ops.logit_params(6, 1.3, 0.5, 0.25)
+        kw = dict(history=i32([1, 1, 2, 7]), history_start=i32([0, 4]), prompt_lens=i32([1]), requests=i32([0] * 6))
+        want, rest = ops.process_logits(x.clone(), prm, **kw), m.clone()
+        assert ops.process_logits(x, prm, out=y, **kw) is y
+        rest[:, y0:y0 + 10] = want
+        assert torch.equal(m, rest)

@@ -1,5 +1,7 @@
 """Refusals of the serving-step operators where arguments lie over one another
 (CPU only, before any device work)."""
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -18,3 +20,14 @@ def test_tree_attention_refuses_an_output_over_its_queries(at, ldq, code):
              nb=1 << 40)
     assert _lib.lib().wl_tree_attention(*a.values(), None) == code
     assert b"overlaps" in _lib.lib().wl_last_error()
+
+
+@pytest.mark.parametrize("at,ld,ldo", [
+    (4, 16, 16), (-4, 16, 16), (36, 16, 16), (28, 16, 16), (64, 16, 16), (64 * 2 + 36, 16, 16), (64, 16, 32),
+    (0, 16, 32), (40, 20, 21), (36, 20, 20), (44, 20, 20),
+])
+def test_process_logits_refuses_an_output_over_other_rows(at, ld, ldo):
+    c = _lib.LogitContext()
+    at += P + 1024
+    assert _lib.lib().wl_process_logits(0, P + 1024, ld, 4, 10, P, C.byref(c), at, ldo, None) == BAD
+    assert b"process_logits: " in _lib.lib().wl_last_error()

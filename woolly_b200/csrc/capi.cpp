@@ -664,6 +664,14 @@ int wl_process_logits(int type, const void* logits, size_t ld, int rows, int voc
   if (!logits || !out || !params) return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: null pointer");
   if (out == logits && ld != ldo)
     return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: in place needs equal row strides");
+  {  // two column ranges of one matrix lie between one another; other overlaps would mix rows
+    const size_t es = type == WL_F32 ? 4 : 2, row = (size_t)vocab * es;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(logits), y = reinterpret_cast<uintptr_t>(out);
+    const size_t apart = (x < y ? y - x : x - y) % (ld * es);
+    if (out != logits && overlap(logits, (rows - 1) * ld * es + row, out, (rows - 1) * ldo * es + row) &&
+        !(ld == ldo && apart >= row && ld * es - apart >= row))
+      return fail(WL_ERR_INVALID_ARGUMENT, "process_logits: out overlaps the logits (it may be the logits themselves)");
+  }
   LogitArgs a;
   a.logits = logits, a.out = out, a.type = type, a.rows = rows, a.vocab = vocab, a.ld = ld, a.ldo = ldo;
   a.params = params, a.ctx = c;
