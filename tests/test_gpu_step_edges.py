@@ -261,3 +261,50 @@ def test_logits_beside_their_output():
         assert ops.process_logits(x, prm, out=y, **kw) is y
         rest[:, y0:y0 + 10] = want
         assert torch.equal(m, rest)
+
+
+FIRST_CALLS = """
+import sys, threading
+sys.path.insert(0, "tests")
+import torch
+from test_gpu_step import BF16, F16, F32, call_attention, make_attention
+from woolly_b200 import ops
+N = 8
+cases = [make_attention(50, [300, 20], [3, 40], 8, 2, hd, qt) for qt in (F32, F16, BF16) for hd in (64, 128, 256)]
+logits = torch.randn(4, 51200, device="cuda")
+torch.cuda.synchronize()
+ready, got, errors = threading.Barrier(N), [None] * N, []
+
+def caller(i):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = []
+            for a in cases:
+                ready.wait()
+                out.append(call_attention(a))
+            ready.wait()
+            out.append(ops.sample(logits, 1.0, 0, 1.0, 0.5))
+            torch.cuda.current_stream().synchronize()
+        got[i] = out
+    except BaseException as e:
+        errors.append(e)
+        ready.abort()
+
+threads = [threading.Thread(target=caller, args=(i,)) for i in range(N)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not errors, errors
+assert all(torch.equal(x, y) for g in got for x, y in zip(g, got[0]))
+"""
+
+
+def test_first_calls_of_many_threads():
+    """Kernels that need their shared memory allowed first, from threads that
+    come at the same time in a process that has not used them."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, timeout=300, capture_output=True, text=True,
+                       env=dict(os.environ, PYTHONPATH=root))
+    assert r.returncode == 0, r.stderr[-3000:]

@@ -298,9 +298,11 @@ __global__ void k_attn_combine(const float* part_o, const float* part_ml, int he
 template <int HD, int G, int TPG>
 int launch_paged_t(const AttnArgs& a, float scale, cudaStream_t st) {
   const size_t smem = (size_t)kRingA * TPG * 2 * kPage * HD * sizeof(__half);
-  if (first_use_on_device((const void*)k_attn_paged<HD, G, TPG>))
+  WL_TRY(once_on_device((const void*)k_attn_paged<HD, G, TPG>, [=]() -> int {
     WL_CUDA_TRY(cudaFuncSetAttribute(k_attn_paged<HD, G, TPG>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    return WL_OK;
+  }));
   return launch_k(k_attn_paged<HD, G, TPG>, dim3(a.kv_heads, a.rows, a.nsplit), dim3(kAttnThreads),
                   smem, st, a, scale);
 }
@@ -575,9 +577,11 @@ __global__ void __launch_bounds__(kPfThreads) k_attn_prefill(const AttnArgs a, f
 template <int HD, int G>
 int launch_prefill_t(const AttnArgs& a, float scale, cudaStream_t st) {
   const size_t smem = (size_t)2 * 2 * kPfKeys * HD * sizeof(__half);
-  if (first_use_on_device((const void*)k_attn_prefill<HD, G>))
+  WL_TRY(once_on_device((const void*)k_attn_prefill<HD, G>, [=]() -> int {
     WL_CUDA_TRY(cudaFuncSetAttribute(k_attn_prefill<HD, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)smem));
+    return WL_OK;
+  }));
   constexpr int CR = 4 * (16 / G);
   return launch_k(k_attn_prefill<HD, G>, dim3((a.rows + CR - 1) / CR, a.kv_heads), dim3(kPfThreads), smem,
                   st, a, scale);

@@ -22,13 +22,16 @@ thread_local std::string g_err;
 void set_error(const std::string& m) { g_err = m; }
 thread_local bool g_pdl = false;
 
-bool first_use_on_device(const void* key) {
+int once_on_device(const void* key, const std::function<int()>& set_up) {
   static std::mutex mu;
   static std::set<std::pair<int, const void*>> seen;
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(mu);
-  return seen.insert({dev, key}).second;
+  if (seen.count({dev, key})) return WL_OK;
+  const int s = set_up();
+  if (s == WL_OK) seen.insert({dev, key});
+  return s;
 }
 bool pdl_enabled() { return g_pdl; }
 void set_pdl(bool on) { g_pdl = on; }

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <functional>
 #include <string>
 
 #include "../../include/woolly_cuda.h"
@@ -12,9 +13,10 @@ namespace wl {
 void set_error(const std::string& msg);
 // programmatic dependent launch for the kernels the calling thread enqueues
 void set_pdl(bool on);
-// true exactly once per (current device, key) across all host threads: guards
-// per-device one-time set-up such as kernel attributes
-bool first_use_on_device(const void* key);
+// set_up() once per (current device, key) across all host threads, such as a
+// kernel's attributes: a thread that comes while another is at it waits for the
+// end, and after a failure the next one tries again
+int once_on_device(const void* key, const std::function<int()>& set_up);
 inline int fail(int code, const std::string& msg) {
   set_error(msg);
   return code;

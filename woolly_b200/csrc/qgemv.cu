@@ -1007,10 +1007,11 @@ int launch_cluster(Kern kern, dim3 grid, int threads, size_t smem, int cx, int c
                    const GemvArgs& a, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (first_use_on_device((const void*)kern)) {
+  WL_TRY(once_on_device((const void*)kern, [=]() -> int {
     WL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
     WL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  }
+    return WL_OK;
+  }));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);

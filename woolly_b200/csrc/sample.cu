@@ -348,9 +348,11 @@ int launch_sample(const float* logits, int rows, int V, int ld, const wl_sample_
     return fail(WL_ERR_INVALID_ARGUMENT,
                 "sample: needs 0 < V <= " + std::to_string(kSampleMaxVocab) + " and ld >= V");
   const size_t smem = (size_t)(V + V / 32 + 1) * sizeof(float);
-  if (first_use_on_device((const void*)k_sample))
+  WL_TRY(once_on_device((const void*)k_sample, []() -> int {
     WL_CUDA_TRY(cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (kSampleMaxVocab + kSampleMaxVocab / 32 + 1) * (int)sizeof(float)));
+    return WL_OK;
+  }));
   return launch_k(k_sample, dim3(rows), dim3(kST), smem, st, logits, V, ld, prm, out);
 }
 

@@ -1413,8 +1413,10 @@ int launch_t(const TreeAttnArgs& a, cudaStream_t st) {
   const int ctas = device_sms();
   const Parts parts = parts_at(a.workspace, ctas, a.n, HD, part_rows(a.rows, a.heads / a.kv_heads));
   constexpr int smem = S::kTiles + (int)sizeof(Small<HD, Q>);
-  if (first_use_on_device((const void*)k_tree_attn<HD, Q>))
+  WL_TRY(once_on_device((const void*)k_tree_attn<HD, Q>, []() -> int {
     WL_CUDA_TRY(cudaFuncSetAttribute(k_tree_attn<HD, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return WL_OK;
+  }));
   WL_TRY(launch_step(k_tree_attn<HD, Q>, dim3(ctas), dim3(kTaThreads), smem, st, a, mk, mv, parts));
   return launch_step(k_tree_combine<HD, Q>, dim3(a.rows, (a.heads + 3) / 4), dim3(128), 0, st, a, parts, ctas);
 }
