@@ -308,3 +308,32 @@ def test_first_calls_of_many_threads():
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, timeout=300, capture_output=True, text=True,
                        env=dict(os.environ, PYTHONPATH=root))
     assert r.returncode == 0, r.stderr[-3000:]
+
+
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 10 ** 12])
+def test_windows_past_every_token(window):
+    """A window beyond 32 bits is none, and not what is left of it."""
+    a = make_attention(51, [300, 40], [3, 20], 4, 2, 64, F16)
+    assert torch.equal(call_attention(a, window), call_attention(a))
+
+
+@pytest.mark.parametrize("hd,repeats", [(64, 256), (128, 128), (256, 64)])
+def test_f32_loses_what_32_products_lose(hd, repeats):
+    """Tensor products cut sums off, towards zero: at the j-th of 32 that are added
+    up in TMEM, up to 2^-23 of what is there, which is j/32 of O: 33/2 x 2^-23 of O
+    together.  (Not half of that on average: each of a product's 16 terms is cut off
+    at the sum's last place, not the sum alone.)  All other roundings are to nearest
+    and cancel over 8,192 keys and hd columns; the last, 2^-24 at most, is counted
+    all the same.  With V positive the mean of the relative error shows the loss; 64
+    products lose twice as much."""
+    a = make_attention(52, [8192], [1], 4, 1, hd, F32)
+    a["q"] /= 4 * math.sqrt(hd / 64)
+    a["cv"] = a["cv"].abs() + 0.5
+    pages = a["tables"][0, :512]
+    k, v = (c[torch.as_tensor(pages, device="cuda")][:, 0].reshape(-1, hd).double() for c in (a["ck"], a["cv"]))
+    want = torch.softmax(a["q"][0].double() @ k.T / math.sqrt(hd), -1) @ v
+    b = dict(a, tables=np.concatenate([np.tile(pages, repeats), [-1]])[None], lengths=np.array([8192 * repeats]),
+             pos=np.array([8192 * repeats]), mask=np.zeros_like(a["mask"]))
+    lost = ((want - call_attention(b)[0].double()) / want).mean().item()
+    print(lost)
+    assert -2.0 ** -24 <= lost <= 33 / 2 * 2.0 ** -23 + 2.0 ** -24

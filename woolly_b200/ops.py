@@ -516,7 +516,7 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
             cache_k.data_ptr(), cache_v.data_ptr(), pages, at, ld, max_pages,
             _i32(lengths, "lengths", (n,), index), _i32(row_start, "row_start", (n + 1,), index),
             _i32(positions, "positions", (rows,), index), m, words or 0, n, rows, heads, kvh, hd,
-            int(window), hd ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), nb)
+            min(int(window), 2 ** 31 - 1), hd ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), nb)
     return out
 
 
