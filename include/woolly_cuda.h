@@ -395,13 +395,19 @@ int wl_kv_commit(int cache_type, const int* tables, int ld_tables, int max_pages
  * negative position, and rows with nothing to attend, give zeros; rows behind
  * row_start[n] are left as they were.  Keys on pages outside the cache are
  * masked.  inf and NaN in K or V reach the rows that attend their token, no
- * others.  out may be q itself, with packed rows (inf and NaN in V then also reach
- * other rows of the request); else it may not overlap it.  q and out are f32 over an f16 cache, or f16 / bf16 over a cache of
- * the same type; head_dim 32, 64, 128 or 256.  f32 queries may have any finite
- * size; at head_dim 64 and above they count with 22 bits of each element, or
- * 2^-39 of the row's largest where that is more.  workspace: wl_tree_attention_workspace
- * bytes of device memory, 16-byte aligned, which the call uses alone until it
- * has finished. */
+ * others.  q and out are f32 over an f16 cache, or f16 / bf16 over a cache of the
+ * same type; head_dim 32, 64, 128 or 256; scale is positive and finite.  out may be
+ * q itself, with packed rows (inf and NaN in V then also reach other rows of the
+ * request); else it may not overlap it.
+ * Sums are held in f32.  f32 queries may have any finite size; at head_dim 64 and
+ * above they and the probabilities count with 22 bits (the queries' elements at
+ * least with 2^-39 of their row's largest), and up to 32 tensor products of 16 keys
+ * go by, each of which may cut 2^-23 off the sum, before it is added up with
+ * rounding: about 2e-6 of the result.  f16 and bf16 queries round each probability
+ * to their type, once, and 512 such products go by.  A wait in the kernel that gives
+ * up, as none does in a sound run, turns the rows concerned into NaN.
+ * workspace: wl_tree_attention_workspace bytes of device memory, 16-byte aligned,
+ * which the call uses alone until it has finished. */
 size_t wl_tree_attention_workspace(int q_type, int n, int rows, int heads, int kv_heads, int head_dim);
 int wl_tree_attention(int q_type, const void* q, size_t ldq, const void* cache_k, const void* cache_v,
                       int n_pages, const int* tables, int ld_tables, int max_pages, const int* lengths,

@@ -25,10 +25,11 @@
 // Counts are integers and of a token's biases the last holds, so atomics' order is
 // not seen.
 //
-// Bound by the copy: 384 drafted rows of 128,000 f32 logits (395 MB) take 118 us =
-// 3.3 TB/s, 52% of the measured copy rate; with every token going through the
+// Bound by the copy: 384 drafted rows of 128,000 f32 logits (395 MB) take 119 us =
+// 3.3 TB/s, 51% of the measured copy rate; with every token going through the
 // rules' branches it was 195 us, row by row with the short lists as marks 187 us.
-// 16 rows of 32,000 take 5.3 us.
+// What is left is the passes over the listed tokens, which follow the CTA's whole
+// copy, at two CTAs per SM.  16 rows of 32,000 take 6.4 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

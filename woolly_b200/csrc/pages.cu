@@ -11,8 +11,8 @@
 // Both are prefix sums over the requests (one CTA, 1024 requests a round, sums
 // in 64 bits) and a scatter over the rows, which starts from a binary search of
 // the rows' prefix sums.  Latency is all there is to them: 64 requests of one
-// token 4.0 us, 32 trees of up to 64 tokens 9.3 us, 1024
-// prompts of 314,000 rows 8.2 us (graph replays).
+// token 4.2 us, 32 trees of up to 64 tokens 9.3 us, 1024 prompts of 314,000 rows
+// 8.6 us (graph replays).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -337,7 +337,7 @@ __device__ __forceinline__ uint4 to_cache(const Eight<C>& e) {
 }
 
 // One thread moves eight values of K and of V.  Bound by memory: 16 rows of 32
-// heads of 128 take 1.6 us in a graph (latency), 16 prompts of up to 512 rows of 8
+// heads of 128 take 1.8 us in a graph (latency), 16 prompts of up to 512 rows of 8
 // heads (50 MB) 9.1 us a call = 5.5 TB/s, 85% of the measured copy rate.
 template <class S, class C>
 __global__ void __launch_bounds__(256) k_kv_append(const S* k, const S* v, size_t ldk, size_t ldv,

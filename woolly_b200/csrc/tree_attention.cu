@@ -39,20 +39,23 @@
 // (f32; 512 for the 16-bit types) it is added, in f32 with rounding, to a copy in
 // the workspace and starts again from zero, while the next scores are on their way:
 // the error does not grow with the context.  f32, 27 requests of 3 tokens over
-// 19,360 keys: 1.3e-6 of the result in 237 us, 1.8e-6 in 226 with 64, 1.2e-5 in 219
-// without.
+// 19,360 keys: 1.2e-6 of the result in 240 us, 1.8e-6 in 229 with 64, 1.2e-5 in 222
+// without.  f16 and bf16 round P once: beside the output's own rounding that is a third
+// of the error more (2.7e-4 of the result for 2.1e-4), and a second word would double
+// the P V products.
 // V rows of keys that no row may see (the end of the last page, a drafted node
 // that is left out, cached tokens below the window) are zeroed in shared memory,
 // since 0 * NaN is not 0.
 //
-// Measured: 8 requests of one token over 32,768 keys, 8 KV heads of 128: 1.07 GB
-// in 206 us = 5.2 TB/s, 81% of the measured copy rate.  32 trees of up to 64
-// tokens over 8,192 keys, 64 / 8 heads of 128, bf16: 414 GFLOP in 742 us = 557
-// TFLOP/s, 32% of the measured GEMM rate.  That is bound by latency: a stream goes
-// scores -> registers -> P -> product -> next scores with TMEM's 512 columns full
-// (two S, two O), so a pair of 128 x 128 tiles takes about 5,000 cycles, of which
-// the tensor pipe works 2,050 and the special-function unit (two exponentials per
-// score pair) 2,100.  Tried and slower: 64-key tiles with two S buffers per stream
+// Measured (graph replays): 8 requests of one token over 32,768 keys, 8 KV heads of
+// 128: 1.07 GB in 209 us = 5.1 TB/s, 79% of the measured copy rate; a ring of three or
+// four tiles instead of five takes as long.  32 trees of up to 64 tokens over 8,192
+// keys, 64 / 8 heads of 128, bf16: 414 GFLOP in 740 to 850 us by box and power = 490
+// to 560 TFLOP/s, 28 to 32% of the measured GEMM rate.  That is bound by latency: a
+// stream goes scores -> registers -> P -> product -> next scores one after the other
+// (TMEM's 512 columns, two S and two O, leave no room for scores ahead), so a pair of
+// 128 x 128 tiles takes about 5,000 cycles, of which the tensor pipe works 2,050 and
+// the special-function unit (two exponentials per score pair) 2,100.  Tried and slower: 64-key tiles with two S buffers per stream
 // (the products of 64 columns cost as much as those of 128), a thread per row with
 // its 128 scores in registers, P taken before the maximum is known, a product warp
 // per stream (both streams' exponentials then fall together), and a third of the
@@ -83,6 +86,10 @@ __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // ---------------------------------------------------------------- one (row, head) per CTA
+// head_dim 32, whose rows are half as wide as the tiles of the tensor kernel: scores a
+// thread per key, in f32, K and V read anew by every (row, head).  Bound by those reads
+// and by a V row being 64 bytes: 16 single tokens over 2,048 keys, 8 heads, 553 us
+// (head_dim 64 on the tensor cores: 36).
 template <class Q, class C>
 __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
   __shared__ float s_q[256], s_p[128], s_red[4];

@@ -485,8 +485,9 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     `scale` defaults to head_dim ** -0.5.
     A row with a negative position or nothing to attend gives zeros; rows
     behind row_start[n] are not written.  q is f32 over an f16 cache, or has
-    the cache's type; head_dim 32, 64, 128 or 256.  `out` may be a packed q,
-    else it may not overlap it."""
+    the cache's type; head_dim 32, 64, 128 or 256.  f16 and bf16 round the
+    probabilities to their type.  `out` may be a packed q, else it may not
+    overlap it."""
     index, pages, kvh, hd, ct = _caches(cache_k, cache_v)
     try:
         qt = q.dtype
@@ -552,7 +553,7 @@ def process_logits(logits: torch.Tensor, params: torch.Tensor, *, history: torch
     bias_values: additive biases; of several for one token the last holds.
     allowed [masks, words]: bit v % 32 of word v // 32 set means token v may
     follow; params' allowed_row picks the mask of each row.  Integers are
-    int32.  `out` may be `logits`."""
+    int32.  `out` may be `logits`, else no row of it may overlap one."""
     try:
         lt = _TYPES.get(logits.dtype)
         rows, V = logits.shape
