@@ -39,10 +39,10 @@
 // (f32; 512 for the 16-bit types) it is added, in f32 with rounding, to a copy in
 // the workspace and starts again from zero, while the next scores are on their way:
 // the error does not grow with the context.  f32, 27 requests of 3 tokens over
-// 19,360 keys: 1.2e-6 of the result in 240 us, 1.8e-6 in 229 with 64, 1.2e-5 in 222
-// without.  f16 and bf16 round P once: beside the output's own rounding that is a third
-// of the error more (2.7e-4 of the result for 2.1e-4), and a second word would double
-// the P V products.
+// 19,360 keys: 1.3e-6 of the result in 237 us, 1.8e-6 in 226 with 64, 1.2e-5 in 219
+// without.  f16 and bf16 round P once, which takes the error, the output's own rounding
+// included, from 2.1e-4 to 2.7e-4 of the result (f16) and from 1.7e-3 to 2.2e-3 (bf16);
+// a second word would double the P V products.
 // V rows of keys that no row may see (the end of the last page, a drafted node
 // that is left out, cached tokens below the window) are zeroed in shared memory,
 // since 0 * NaN is not 0.
@@ -55,11 +55,11 @@
 // stream goes scores -> registers -> P -> product -> next scores one after the other
 // (TMEM's 512 columns, two S and two O, leave no room for scores ahead), so a pair of
 // 128 x 128 tiles takes about 5,000 cycles, of which the tensor pipe works 2,050 and
-// the special-function unit (two exponentials per score pair) 2,100.  Tried and slower: 64-key tiles with two S buffers per stream
-// (the products of 64 columns cost as much as those of 128), a thread per row with
-// its 128 scores in registers, P taken before the maximum is known, a product warp
-// per stream (both streams' exponentials then fall together), and a third of the
-// exponentials as polynomials on the FMA pipe.
+// the special-function unit (two exponentials per score pair) 2,100.  Tried and
+// slower: 64-key tiles with two S buffers per stream (the products of 64 columns cost
+// as much as those of 128), a thread per row with its 128 scores in registers, P taken
+// before the maximum is known, a product warp per stream (both streams' exponentials
+// then fall together), and a third of the exponentials as polynomials on the FMA pipe.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -86,10 +86,10 @@ __device__ __forceinline__ void put(__half* p, float x) { *p = __float2half_rn(x
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // ---------------------------------------------------------------- one (row, head) per CTA
-// head_dim 32, whose rows are half as wide as the tiles of the tensor kernel: scores a
-// thread per key, in f32, K and V read anew by every (row, head).  Bound by those reads
-// and by a V row being 64 bytes: 16 single tokens over 2,048 keys, 8 heads, 553 us
-// (head_dim 64 on the tensor cores: 36).
+// head_dim 32, whose rows are half as wide as the tiles of the tensor kernel: a thread
+// per key for the scores, in f32, then 32 of the 128 threads for V, a column each, key
+// after key; K and V read anew by every (row, head).  Bound by that serial pass: 16
+// single tokens over 2,048 keys, 8 heads, 553 us (head_dim 64 on the tensor cores: 36).
 template <class Q, class C>
 __global__ void __launch_bounds__(128) k_tree_attn_row(const TreeAttnArgs a) {
   __shared__ float s_q[256], s_p[128], s_red[4];
